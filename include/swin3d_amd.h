@@ -701,6 +701,76 @@ int s3d_swin_block_grad(const s3d_block_saved *saved, const s3d_block_gradients 
                         int32_t H, int32_t D, int32_t hidden, const int32_t *table_sizes, int32_t nd, int64_t table_len, int64_t W,
                         int64_t pairs, float q_scale, int32_t dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Rows in eight bits for products in whole numbers: codes device int8 [N,C] and scales device fp32 [N], of y
+ *   s = x + residual (fp32);  y = (s - mean(s)) / sqrt(var(s) + eps) * gamma + beta,  or with rms  s / sqrt(mean(s^2) + eps) * gamma
+ *   scale = max |y| / 127;    code = 127 y / max |y| to the nearest, ties to even
+ * A row of zeros has scale 0; one with a number that is not finite has codes 0 and scale NaN.
+ *   x              device fp32 [N,C];  residual: device [N,C] of residual_dtype, or null
+ *   gamma, beta    device fp32 [C], or null (ones, zeros); beta is not read with rms
+ *   sum            device fp32 [N,C] for s, x itself or apart, or null; not written without a residual
+ * Dense and 16-byte aligned; C a multiple of 4 up to 8192; arithmetic in fp32.
+ */
+int s3d_add_norm_int8(const float *x, const void *residual, int32_t residual_dtype, const float *gamma, const float *beta, float eps,
+                      int32_t rms, float *sum, int8_t *codes, float *scales, int64_t N, int32_t C, void *stream);
+/* the same of rows as they are, in fp32 or fp16 (`dtype`): those of an attention or a GELU, and weights (a scale per output channel) */
+int s3d_quantize_rows(const void *x, int32_t dtype, int8_t *codes, float *scales, int64_t N, int32_t C, void *stream);
+/* out [N,C] of `dtype`: what such rows stand for, code times scale */
+int s3d_int8_values(const int8_t *codes, const float *scales, void *out, int32_t dtype, int64_t N, int32_t C, void *stream);
+
+/*
+ * y = x w^T + bias of such rows (x [M,K] with x_scales [M], w [N,K] with w_scales [N]), then GELU where gelu is not zero: sums
+ * of whole numbers in 32 bits, scales, bias (fp32 [N] or null) and GELU in fp32, one rounding to fp16.  Dense and 16-byte aligned;
+ * N a multiple of 8, K of 16 and at most 65536.
+ */
+int s3d_linear_int8(const int8_t *x, const float *x_scales, const int8_t *w, const float *w_scales, const float *bias, void *y, int64_t M,
+                    int32_t N, int32_t K, int32_t gelu, void *stream);
+/*
+ * Both layers of an MLP: u = fp16(GELU(x w1^T + b1)), in eight bits as s3d_quantize_rows has them, then y = u w2^T + b2, fp16
+ * [M,C].  C and hidden multiples of 16, at most 8192.
+ */
+size_t s3d_mlp_int8_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
+int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const float *w1_scales, const float *b1, const int8_t *w2,
+                 const float *w2_scales, const float *b2, void *y, int64_t M, int32_t C, int32_t hidden, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/*
+ * Kept rows: what the backward of a layer reads of its fp16 input, in 1.0625 bytes a number.  Sixteen neighbouring numbers of a row
+ * share a scale, the smallest number of four significant bits and multiple of 2^-24 with 127 scales reaching the largest of them;
+ * code = x / scale to the nearest, ties to even.  What a code stands for, code times scale, is an fp16 number (at the largest scale,
+ * 576, codes end at 113 for that).  A group with a number that is not finite stands for NaN.
+ *   kept   device [s3d_kept_bytes(M, K)]: int8 codes [M,K], then a byte per group [M, K / 16]: three bits of mantissa below five of
+ *          an exponent e, (8 + mantissa) 2^(e - 25), or mantissa 2^-24 for e = 0; 255 for NaN
+ * K a multiple of 16 up to 16384; 16-byte aligned.
+ */
+size_t s3d_kept_bytes(int64_t M, int32_t K);
+int s3d_keep_rows(const void *x, void *kept, int64_t M, int32_t K, void *stream);
+/* out fp16 [M,K]: what kept rows stand for */
+int s3d_kept_values(const void *kept, void *out, int64_t M, int32_t K, void *stream);
+
+/*
+ * A dense layer in training that keeps its input in that form: y = x w^T + bias (fp16 [M,K], [N,K], [N] or null, [M,N]) and, unless
+ * null, kept of x.  Its gradients: dx = dy w (w_t: the weight transposed, fp16 [K,N]), dw = dy^T x' and db = the column sums of dy in
+ * grad_dtype, x' what kept stands for; those that are null are left out, with kept unless dw is wanted and w_t unless dx is.  M at least
+ * 1, N and K multiples of 16 up to 16384; dense and 16-byte aligned.  The same bits on every call.
+ */
+int s3d_kept_linear(const void *x, const void *w, const void *bias, void *y, void *kept, int64_t M, int32_t N, int32_t K, void *stream);
+size_t s3d_kept_linear_grad_workspace_bytes(int64_t M, int32_t N, int32_t K);
+int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void *dx, void *dw, void *db, int32_t grad_dtype, int64_t M,
+                         int32_t N, int32_t K, void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * An MLP likewise: h = x w1^T + b1 (rounded to fp16), y = GELU(h) w2^T + b2, x and h kept (each unless null).  Its gradients, h' and x'
+ * what is kept: dh = (dy w2) GELU'(h'), dw2 = dy^T GELU(h'), db2 = column sums of dy, dx = dh w1, dw1 = dh^T x', db1 = column sums of dh,
+ * each unless null.  Nothing of the hidden layer's size in fp16 outlives a call.
+ */
+size_t s3d_kept_mlp_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
+int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *y, void *kept_x, void *kept_h,
+                 int64_t M, int32_t C, int32_t hidden, void *workspace, size_t workspace_bytes, void *stream);
+size_t s3d_kept_mlp_grad_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
+int s3d_kept_mlp_grad(const void *dy, const void *w1_t, const void *w2_t, const void *kept_x, const void *kept_h, void *dx, void *dw1,
+                      void *db1, void *dw2, void *db2, int32_t grad_dtype, int64_t M, int32_t C, int32_t hidden, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

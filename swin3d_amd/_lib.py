@@ -136,6 +136,22 @@ SIGNATURES = {
     "s3d_mlp": (ctypes.c_int, [_vp] * 6 + [_i64, _i32, _i32, _vp]),
     "s3d_linear_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
     "s3d_linear_grad": (ctypes.c_int, [_vp] * 4 + [_i32, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_add_norm_int8": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, ctypes.c_float, _i32, _vp, _vp, _vp, _i64, _i32, _vp]),
+    "s3d_quantize_rows": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i32, _vp]),
+    "s3d_int8_values": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i64, _i32, _vp]),
+    "s3d_linear_int8": (ctypes.c_int, [_vp] * 6 + [_i64, _i32, _i32, _i32, _vp]),
+    "s3d_mlp_int8_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
+    "s3d_mlp_int8": (ctypes.c_int, [_vp] * 9 + [_i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_kept_bytes": (ctypes.c_size_t, [_i64, _i32]),
+    "s3d_keep_rows": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
+    "s3d_kept_values": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
+    "s3d_kept_linear": (ctypes.c_int, [_vp] * 5 + [_i64, _i32, _i32, _vp]),
+    "s3d_kept_linear_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
+    "s3d_kept_linear_grad": (ctypes.c_int, [_vp] * 6 + [_i32, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_kept_mlp_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
+    "s3d_kept_mlp": (ctypes.c_int, [_vp] * 8 + [_i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_kept_mlp_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
+    "s3d_kept_mlp_grad": (ctypes.c_int, [_vp] * 10 + [_i32, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
     "s3d_swin_blocks_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
     # x x_out pending | N H D hidden | table sizes nd len | sets blocks | ws bytes stream
     "s3d_swin_blocks": (ctypes.c_int, [_vp] * 3 + [_i64, _i32, _i32, _i32] + [_vp, _i32, _i64] + [_vp, _i32] * 2 +

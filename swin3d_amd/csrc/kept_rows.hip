@@ -1,0 +1,259 @@
+// Dense layers in training that keep what their backward reads of their input in eight bits (gfx950); rows8.h has the form.
+//
+//   linear   y = x W^T + b;                       dx = dy W;  dW = dy^T x';  db = column sums of dy
+//   MLP      h = x W1^T + b1;  y = GELU(h) W2^T + b2;
+//            dh = (dy W2) GELU'(h');  dW2 = dy^T GELU(h');  dx = dh W1;  dW1 = dh^T x';  db2, db1 = column sums of dy, dh
+//
+// with x', h' what is kept of x and h (rounded to fp16).  Products of fp16 operands with sums in fp32; GELU(h') and dh are rounded to
+// fp16 for the products behind them.  Of an MLP with hidden = 4 C that leaves 5.3 C bytes a row for the backward, where x, h and GELU(h)
+// in fp16 are 18 C.
+#include "linear.h"
+#include "rows8.h"
+
+namespace s3d {
+namespace {
+
+constexpr int kThreads = 256;
+
+__host__ __device__ inline size_t codes_bytes(int64_t M, int32_t K) { return static_cast<size_t>(M) * K; }
+
+// a group a thread
+__global__ __launch_bounds__(kThreads) void keep_kernel(const _Float16 *__restrict__ x, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, int64_t groups)
+{
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < groups; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const half8 lo = reinterpret_cast<const half8 *>(x)[2 * i], hi = reinterpret_cast<const half8 *>(x)[2 * i + 1];
+        const uint32_t byte = kept_byte(max(largest_bits(lo), largest_bits(hi)));
+        const Divisor d(byte);
+        const uint2 a = kept_codes(lo, d), b = kept_codes(hi, d);
+        reinterpret_cast<uint4 *>(codes)[i] = make_uint4(a.x, a.y, b.x, b.y);
+        scales[i] = static_cast<uint8_t>(byte);
+    }
+}
+
+// x Phi(x) as the forward has it
+__device__ __forceinline__ half8 gelu_of(const half8 &v)
+{
+    half8 u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = static_cast<_Float16>(gelu(v[e]));
+    return u;
+}
+
+// half a group a thread: what the codes stand for to `out`, GELU of it to `active`; either may be null
+__global__ __launch_bounds__(kThreads) void kept_values_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, _Float16 *__restrict__ out,
+                                                               _Float16 *__restrict__ active, int64_t pieces)
+{
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const half8 v = kept_numbers(reinterpret_cast<const uint2 *>(codes)[i], scales[i / 2]);
+        if (out) reinterpret_cast<half8 *>(out)[i] = v;
+        if (active) reinterpret_cast<half8 *>(active)[i] = gelu_of(v);
+    }
+}
+
+dim3 grid_of(int64_t threads)
+{
+    const int64_t blocks = ceil_div(threads, kThreads);
+    return dim3(static_cast<unsigned>(blocks < (1 << 22) ? blocks : 1 << 22));
+}
+
+bool rows_fit(int64_t M, int32_t K) { return M >= 0 && M <= 0x7fffffff && K >= 16 && K % 16 == 0 && K <= 16384; }
+// (M = 0 has no gradients to speak of; the callers return zeros)
+bool fits(int64_t M, int32_t N, int32_t K) { return rows_fit(M, K) && M >= 1 && N >= 16 && N % 16 == 0 && N <= 16384; }
+int bad_shape(const char *who, int64_t M, int32_t N, int32_t K)
+{
+    return fail(S3D_ERR_BAD_SHAPE, "%s: M=%lld, widths %d and %d (M at least 1, widths multiples of 16, at most 16384)", who, (long long)M, K, N);
+}
+
+int keep(const void *x, void *kept, int64_t M, int32_t K, hipStream_t stream)
+{
+    uint8_t *codes = static_cast<uint8_t *>(kept);
+    const int64_t groups = M * (K / kKeptGroup);
+    hipLaunchKernelGGL(keep_kernel, grid_of(groups), dim3(kThreads), 0, stream, static_cast<const _Float16 *>(x), codes, codes + codes_bytes(M, K), groups);
+    S3D_HIP_CHECK(hipGetLastError());
+    return S3D_OK;
+}
+
+int values(const void *kept, void *out, void *active, int64_t M, int32_t K, hipStream_t stream)
+{
+    const uint8_t *codes = static_cast<const uint8_t *>(kept);
+    const int64_t pieces = M * (K / 8);
+    hipLaunchKernelGGL(kept_values_kernel, grid_of(pieces), dim3(kThreads), 0, stream, codes, codes + codes_bytes(M, K), static_cast<_Float16 *>(out),
+                       static_cast<_Float16 *>(active), pieces);
+    S3D_HIP_CHECK(hipGetLastError());
+    return S3D_OK;
+}
+
+// x' and the parts of the weight's gradient
+struct LinearPlaces {
+    size_t x, parts, total;
+};
+LinearPlaces linear_places(int64_t M, int32_t N, int32_t K)
+{
+    LinearPlaces p{};
+    const LinearGrad g{nullptr, nullptr, nullptr, nullptr, M, N, K, 0, 1.0f};
+    p.parts = align_up(2 * codes_bytes(M, K), 256);
+    p.total = p.parts + linear_grads_bytes(&g, 1);
+    return p;
+}
+
+struct MlpLayers {
+    LinearGrad of[2];      // fc2, fc1
+};
+MlpLayers mlp_layers(int64_t M, int32_t C, int32_t hidden)
+{
+    return {{{nullptr, nullptr, nullptr, nullptr, M, C, hidden, 0, 1.0f}, {nullptr, nullptr, nullptr, nullptr, M, hidden, C, 0, 1.0f}}};
+}
+// x', h', GELU(h') and dh, and the parts of the weights' gradients
+struct MlpPlaces {
+    size_t x, hidden, active, dhidden, parts, total;
+};
+MlpPlaces mlp_places(int64_t M, int32_t C, int32_t hidden)
+{
+    MlpPlaces p{};
+    const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
+    const MlpLayers layers = mlp_layers(M, C, hidden);
+    p.hidden = align_up(2 * codes_bytes(M, C), 256);
+    p.active = p.hidden + wide;
+    p.dhidden = p.active + wide;
+    p.parts = p.dhidden + wide;
+    p.total = p.parts + linear_grads_bytes(layers.of, 2);
+    return p;
+}
+
+}  // namespace
+}  // namespace s3d
+
+using namespace s3d;
+
+extern "C" __attribute__((visibility("default"))) size_t s3d_kept_bytes(int64_t M, int32_t K)
+{
+    return rows_fit(M, K) ? codes_bytes(M, K) + codes_bytes(M, K) / kKeptGroup : 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_keep_rows(const void *x, void *kept, int64_t M, int32_t K, void *stream)
+{
+    if (!rows_fit(M, K)) return fail(S3D_ERR_BAD_SHAPE, "s3d_keep_rows: M=%lld K=%d (K a multiple of 16, at most 16384)", (long long)M, K);
+    if (M == 0) return S3D_OK;
+    if (!x || !kept) return fail(S3D_ERR_NULL_POINTER, "s3d_keep_rows: null device pointer");
+    return keep(x, kept, M, K, static_cast<hipStream_t>(stream));
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_values(const void *kept, void *out, int64_t M, int32_t K, void *stream)
+{
+    if (!rows_fit(M, K)) return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_values: M=%lld K=%d (K a multiple of 16, at most 16384)", (long long)M, K);
+    if (M == 0) return S3D_OK;
+    if (!kept || !out) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_values: null device pointer");
+    return values(kept, out, nullptr, M, K, static_cast<hipStream_t>(stream));
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void *x, const void *w, const void *bias, void *y, void *kept, int64_t M, int32_t N,
+                                                                      int32_t K, void *stream)
+{
+    if (!fits(M, N, K)) return bad_shape("s3d_kept_linear", M, N, K);
+    if (!x || !w || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear: null device pointer");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (kept)
+        if (int rc = keep(x, kept, M, K, s)) return rc;
+    return launch_linear({x, w, bias, y, M, N, K, false}, s);
+}
+
+extern "C" __attribute__((visibility("default"))) size_t s3d_kept_linear_grad_workspace_bytes(int64_t M, int32_t N, int32_t K)
+{
+    return fits(M, N, K) ? linear_places(M, N, K).total : 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void *dx, void *dw, void *db,
+                                                                           int32_t grad_dtype, int64_t M, int32_t N, int32_t K, void *workspace,
+                                                                           size_t workspace_bytes, void *stream)
+{
+    if (!fits(M, N, K)) return bad_shape("s3d_kept_linear_grad", M, N, K);
+    if (grad_dtype != S3D_DTYPE_F32 && grad_dtype != S3D_DTYPE_F16)
+        return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_linear_grad: grad_dtype %d (0 = fp32, 1 = fp16)", grad_dtype);
+    if (!dy || (dx && !w_t) || (dw && !kept)) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear_grad: null device pointer");
+    const LinearPlaces p = linear_places(M, N, K);
+    if (!workspace || workspace_bytes < p.total)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_linear_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);
+    char *base = static_cast<char *>(workspace);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dx)
+        if (int rc = launch_linear({dy, w_t, nullptr, dx, M, K, N, false}, s)) return rc;
+    if (!dw && !db) return S3D_OK;
+    if (dw) {
+        if (int rc = values(kept, base + p.x, nullptr, M, K, s)) return rc;
+    }
+    // (for the bias alone the other operand is any rows)
+    LinearGrad g{dy, dw ? base + p.x : dy, dw, db, M, N, dw ? K : 16, 0, 1.0f};
+    float *parts = reinterpret_cast<float *>(base + p.parts);
+    if (int rc = launch_linear_grad_parts(&g, 1, &parts, s)) return rc;
+    return launch_linear_grad_sums(&g, 1, nullptr, grad_dtype, s);
+}
+
+extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
+{
+    return fits(M, hidden, C) ? 2 * align_up(2 * codes_bytes(M, hidden), 256) : 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *y,
+                                                                   void *kept_x, void *kept_h, int64_t M, int32_t C, int32_t hidden, void *workspace,
+                                                                   size_t workspace_bytes, void *stream)
+{
+    if (!fits(M, hidden, C)) return bad_shape("s3d_kept_mlp", M, hidden, C);
+    if (!x || !w1 || !w2 || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_mlp: null device pointer");
+    const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
+    if (!workspace || workspace_bytes < 2 * wide)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), 2 * wide);
+    char *h = static_cast<char *>(workspace), *active = h + wide;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (kept_x)
+        if (int rc = keep(x, kept_x, M, C, s)) return rc;
+    LinearArgs first{x, w1, b1, h, M, hidden, C, false};
+    first.in_order = true;
+    first.gelu_out = active;
+    if (int rc = launch_linear(first, s)) return rc;
+    if (kept_h)
+        if (int rc = keep(h, kept_h, M, hidden, s)) return rc;
+    return launch_linear({active, w2, b2, y, M, C, hidden, false}, s);
+}
+
+extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_grad_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
+{
+    return fits(M, hidden, C) ? mlp_places(M, C, hidden).total : 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const void *dy, const void *w1_t, const void *w2_t, const void *kept_x,
+                                                                        const void *kept_h, void *dx, void *dw1, void *db1, void *dw2, void *db2,
+                                                                        int32_t grad_dtype, int64_t M, int32_t C, int32_t hidden, void *workspace,
+                                                                        size_t workspace_bytes, void *stream)
+{
+    if (!fits(M, hidden, C)) return bad_shape("s3d_kept_mlp_grad", M, hidden, C);
+    if (grad_dtype != S3D_DTYPE_F32 && grad_dtype != S3D_DTYPE_F16)
+        return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_mlp_grad: grad_dtype %d (0 = fp32, 1 = fp16)", grad_dtype);
+    const bool behind = dx || dw1 || db1;      // the gradients behind that of the hidden layer
+    if (!dy || ((behind || dw2) && !kept_h) || (behind && !w2_t) || (dx && !w1_t) || (dw1 && !kept_x))
+        return fail(S3D_ERR_NULL_POINTER, "s3d_kept_mlp_grad: null device pointer");
+    const MlpPlaces p = mlp_places(M, C, hidden);
+    if (!workspace || workspace_bytes < p.total)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);
+    char *base = static_cast<char *>(workspace), *active = base + p.active, *dhidden = base + p.dhidden;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (behind || dw2)
+        if (int rc = values(kept_h, behind ? base + p.hidden : nullptr, dw2 ? active : nullptr, M, hidden, s)) return rc;
+    LinearGrad grads[2];
+    int num = 0;
+    if (dw2 || db2) grads[num++] = LinearGrad{dy, dw2 ? active : dy, dw2, db2, M, C, dw2 ? hidden : 16, 0, 1.0f};
+    if (behind) {
+        LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false, base + p.hidden};
+        if (int rc = launch_linear(a, s)) return rc;
+        if (dx)
+            if (int rc = launch_linear({dhidden, w1_t, nullptr, dx, M, C, hidden, false}, s)) return rc;
+    }
+    if (dw1 || db1) {
+        if (dw1)
+            if (int rc = values(kept_x, base + p.x, nullptr, M, C, s)) return rc;
+        grads[num++] = LinearGrad{dhidden, dw1 ? static_cast<const void *>(base + p.x) : dhidden, dw1, db1, M, hidden, dw1 ? C : 16, 0, 1.0f};
+    }
+    if (num == 0) return S3D_OK;
+    float *parts = reinterpret_cast<float *>(base + p.parts);
+    if (int rc = launch_linear_grad_parts(grads, num, &parts, s)) return rc;
+    return launch_linear_grad_sums(grads, num, nullptr, grad_dtype, s);
+}

@@ -29,6 +29,19 @@ bool mlp_takes(int64_t M, int32_t C, int32_t hidden);
 bool mlp_pays(int64_t M, int32_t C, int32_t hidden);      // ... and is faster than the layers apart
 int launch_mlp(const MlpArgs &a, hipStream_t stream);
 
+// Dense layers of rows in eight bits (linear_int8.hip)
+struct LinearInt8 {
+    const int8_t *x, *w;              // [M,K], [N,K]
+    const float *sx, *sw, *bias;      // [M], [N], [N] or null
+    void *y;                          // [M,N] fp16
+    int64_t M;
+    int32_t N, K;
+    bool gelu;
+};
+int launch_linear_int8(const LinearInt8 &l, hipStream_t stream);
+// Rows of fp32 or fp16 in eight bits with a scale each (norm_int8.hip)
+int launch_quantize_rows(const void *x, int32_t dtype, int8_t *codes, float *scales, int64_t N, int32_t C, hipStream_t stream);
+
 // A layer's weight and bias gradients (linear_grad.hip): dw = dy^T x, db = the column sums of dy; the first `scaled` rows of
 // the weight (and numbers of the bias) are parameters times `scale`
 struct LinearGrad {

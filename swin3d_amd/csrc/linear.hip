@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 64;        // numbers of K staged at a time
-constexpr int kPieces = kChunk / 8;
+static_assert(kChunk / 8 == kPieces, "pieces of eight numbers");
 
 // The derivative of x Phi(x): Phi(x) + x phi(x), in fp32.  With Phi(-u) = phi(u) M(u), M the ratio of Mills, that is
 // phi(u) (u - M(u)) with the sign of x, and 1 more for x above 0, u = |x|: u - M(u) by the polynomial of degree 12 that fits
@@ -57,23 +57,6 @@ __device__ __forceinline__ float gelu_slope(float x)
 __device__ __forceinline__ float gelu_erf(float x) { return (x * 0.5f) * (1.0f + erff(x * 0.70710678f)); }
 
 enum class Behind { kNothing, kGelu, kGeluGrad, kGeluBeside };
-
-// The place of 16-byte piece p of row r: sixteen consecutive rows' pieces p lie in 64 different banks.
-__device__ __forceinline__ int placed(int r, int p) { return r * kPieces + (p ^ ((r >> 1) & (kPieces - 1))); }
-
-// Sixteen bytes a lane from `from` to the wavefront's 1024 at `to` in LDS.  The compiler knows nothing of them: who reads them
-// has waited for them (loads and stores end in the order of their issue) and met the other wavefronts at a barrier.  (m0 is reserved,
-// of which it warns; named, it is a definition of m0, which the compiler's own uses of it have to respect.)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load_to_lds(uint32_t to, const void *from)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0", "memory");
-}
-#pragma clang diagnostic pop
-// ... all but the kBehind instructions issued last
-template <int kBehind> __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kBehind) : "memory"); }
-__device__ __forceinline__ void workgroup_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // WM x WN wavefronts of TM x TN products of 32 x 32
 template <int WM, int WN, int TM, int TN> struct Tile {

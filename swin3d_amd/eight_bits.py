@@ -1,0 +1,404 @@
+"""Dense layers whose rows are held in eight bits.
+
+At inference a layer's input is whole numbers with a scale a row (`Int8Rows`), its weight whole numbers with a scale an output
+channel, and the product a sum of whole numbers, exact, with both scales behind it:
+
+    sum, rows = add_norm_int8(x, branch, block.norm2)           # (x + branch, its LayerNorm or RMSNorm in eight bits)
+    y = linear_int8(rows, quantize_rows(layer.weight), layer.bias)
+    y = mlp_int8(rows, quantize_rows(fc1.weight), fc1.bias, quantize_rows(fc2.weight), fc2.bias)
+
+In training a layer keeps what its backward reads of its input in eight bits, in groups of sixteen numbers with a scale each
+(`keep_rows`): the forward is the layer's own in fp16, and so is the gradient of its input; the weight's gradient is that of rows a 254th of
+their group's largest number off at most, and an eighth of that more where a scale of four bits is above what the group needs:
+
+    y = checkpointed_linear(x, layer.weight, layer.bias)
+    y = checkpointed_mlp(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias)
+
+`swin3d_amd.encoder.eight_bit_inference` and `eight_bit_checkpoints` make the blocks of a network use them.
+
+All take dense CUDA (HIP) tensors, enqueue on torch's current stream of their device and do not wait.  What is wrong with an argument
+raises ValueError, CPU tensors included.
+"""
+from typing import NamedTuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import Function, once_differentiable
+
+from . import _lib
+from .linear_grad import _half_copies
+from .swin_blocks import followed
+
+_DTYPE_CODE = {torch.float32: _lib.S3D_DTYPE_F32, torch.float16: _lib.S3D_DTYPE_F16}
+_MOST_CHANNELS, _MOST_SUMMED, _MOST_WIDTH, _MOST_HIDDEN = 8192, 65536, 16384, 8192
+
+
+class Int8Rows(NamedTuple):
+    """Rows in eight bits: codes int8 [N,C], scales float32 [N]; row i stands for codes[i] * scales[i]."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def values(self, dtype=torch.float16):
+        """[N,C] in float16 or float32: what the rows stand for."""
+        _check_rows("rows", self)
+        if dtype not in _DTYPE_CODE:
+            raise ValueError(f"dtype {dtype} (float16 or float32)")
+        n, c = self.codes.shape
+        if c == 0 or c % 4 or c > _MOST_CHANNELS:
+            raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
+        dev = self.codes.device
+        codes, scales = _dense(self.codes), self.scales.contiguous()
+        out = torch.empty((n, c), dtype=dtype, device=dev)
+        with _lib.on(dev):
+            status = _lib.lib().s3d_int8_values(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), _DTYPE_CODE[dtype], n, c, _lib.stream(dev))
+        _lib.check(status, "s3d_int8_values")
+        return out
+
+
+def _dense(t):
+    """t as the kernels read it: dense and 16-byte aligned."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check(name, t, dtypes, shape, device=None):
+    """t is a plain tensor on the GPU (on `device`) of one of the dtypes and of `shape`, in which None stands for any size."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
+    if not t.is_cuda or t.dtype not in dtypes or t.dim() != len(shape) or any(s is not None and s != got for s, got in zip(shape, t.shape)) \
+            or (device is not None and t.device != device):
+        sizes = ",".join("any" if s is None else str(s) for s in shape)
+        kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+        where = "on a CUDA (HIP) device" if device is None else f"on {device}"
+        raise ValueError(f"{name} must be {kinds} [{sizes}] {where}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dim() and t.shape[0] > 0x7fffffff:
+        raise ValueError(f"{name} has {t.shape[0]} rows (at most 2^31 - 1)")
+
+
+def _check_rows(name, rows, device=None):
+    if not isinstance(rows, tuple) or len(rows) != 2:
+        raise ValueError(f"{name} must be Int8Rows, got {type(rows).__name__}")
+    codes, scales = rows
+    _check(f"{name}.codes", codes, (torch.int8,), (None, None), device)
+    _check(f"{name}.scales", scales, (torch.float32,), (codes.shape[0],), codes.device)
+
+
+def _unfollowed(what, *tensors):
+    """These calls are no operations of autograd: nothing may follow them."""
+    if followed():
+        raise RuntimeError(f"{what} does not run under a transform, a forward-mode derivative, a dispatch mode or a tracer")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach what requires one")
+
+
+def _empty_rows(n, c, device):
+    return Int8Rows(torch.empty((n, c), dtype=torch.int8, device=device), torch.empty(n, dtype=torch.float32, device=device))
+
+
+def add_norm_int8(x, residual, norm, inplace=False):
+    """(x + residual, norm(x + residual) in eight bits) for x fp32 [N,C] and `norm` a torch.nn.LayerNorm or RMSNorm over C.
+
+    residual   fp16 / fp32 [N,C] or None (then the first result is x itself)
+    inplace    write the sum back into x instead of a new tensor
+    C is a multiple of 4 and at most 8192.  A row with a number that is not finite stands for NaN.  No autograd.
+    """
+    _check("x", x, (torch.float32,), (None, None))
+    n, c = x.shape
+    dev = x.device
+    if c == 0 or c % 4 or c > _MOST_CHANNELS:
+        raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
+    rms = isinstance(norm, nn.RMSNorm)
+    if not (rms or isinstance(norm, nn.LayerNorm)) or tuple(norm.normalized_shape) != (c,):
+        raise ValueError(f"norm must be a LayerNorm or RMSNorm over the {c} channels, got {norm}")
+    weight, bias = norm.weight, None if rms else norm.bias
+    for name, p in (("norm.weight", weight), ("norm.bias", bias)):
+        if p is not None:
+            _check(name, p, (torch.float32, torch.float16, torch.bfloat16, torch.float64), (c,), dev)
+    if residual is not None:
+        _check("residual", residual, tuple(_DTYPE_CODE), (n, c), dev)
+    _unfollowed("add_norm_int8", x, residual, weight, bias)
+    if inplace and residual is not None and not (x.is_contiguous() and x.data_ptr() % 16 == 0):
+        raise ValueError("x must be contiguous and 16-byte aligned to be written in place")
+    eps = norm.eps if norm.eps is not None else torch.finfo(torch.float32).eps
+    rows_in = _dense(x)
+    res_ptr, res_code, summed = None, 0, x
+    if residual is not None:
+        residual = _dense(residual)
+        res_ptr, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]
+        summed = x if inplace else torch.empty((n, c), dtype=torch.float32, device=dev)
+    gamma, beta = (None if p is None else _dense(p.detach().float()) for p in (weight, bias))
+    rows = _empty_rows(n, c, dev)
+    with _lib.on(dev):
+        status = _lib.lib().s3d_add_norm_int8(
+            rows_in.data_ptr(), res_ptr, res_code, None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), float(eps),
+            int(rms), None if residual is None else summed.data_ptr(), rows.codes.data_ptr(), rows.scales.data_ptr(), n, c, _lib.stream(dev))
+    _lib.check(status, "s3d_add_norm_int8")
+    return summed, rows
+
+
+def quantize_rows(x):
+    """Int8Rows of fp16 or fp32 rows [N,C]: the input of a layer, or a weight [out,in].  scale = max |row| / 127, code = row / scale to the
+    nearest, ties to even.  C is a multiple of 4 and at most 8192.  No autograd: x is taken as its data."""
+    _check("x", x, tuple(_DTYPE_CODE), (None, None))
+    n, c = x.shape
+    if c == 0 or c % 4 or c > _MOST_CHANNELS:
+        raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
+    _unfollowed("quantize_rows")
+    x = _dense(x.detach())
+    rows = _empty_rows(n, c, x.device)
+    with _lib.on(x.device):
+        status = _lib.lib().s3d_quantize_rows(x.data_ptr(), _DTYPE_CODE[x.dtype], rows.codes.data_ptr(), rows.scales.data_ptr(), n, c,
+                                              _lib.stream(x.device))
+    _lib.check(status, "s3d_quantize_rows")
+    return rows
+
+
+def _layer_operands(name, weight, bias, k, dev):
+    """(codes, scales, bias or None) of a layer of k inputs, as the kernels read them."""
+    _check_rows(name, weight, dev)
+    n = weight.codes.shape[0]
+    if weight.codes.shape[1] != k:
+        raise ValueError(f"{name} takes {weight.codes.shape[1]} channels, the rows have {k}")
+    if bias is not None:
+        _check(f"the bias of {name}", bias, (torch.float32, torch.float16), (n,), dev)
+        bias = _dense(bias.detach().float())
+    return _dense(weight.codes), _dense(weight.scales), bias
+
+
+def linear_int8(rows, weight, bias=None, gelu=False):
+    """fp16 [N,out]: rows @ weight.T + bias, then GELU (the exact form) where `gelu`.
+
+    rows     Int8Rows [N,in]: of add_norm_int8 or quantize_rows
+    weight   Int8Rows [out,in]: quantize_rows(layer.weight)
+    bias     fp32 or fp16 [out], or None
+    The sums are exact, scales, bias and GELU fp32, with one rounding at the end.  in is a multiple of 16 up to 65536, out of 8.  No autograd.
+    """
+    _check_rows("rows", rows)
+    m, k = rows.codes.shape
+    dev = rows.codes.device
+    w, sw, bias = _layer_operands("weight", weight, bias, k, dev)
+    n = w.shape[0]
+    if k == 0 or k % 16 or k > _MOST_SUMMED or n == 0 or n % 8:
+        raise ValueError(f"a layer from {k} to {n} channels (from a multiple of 16 up to {_MOST_SUMMED}, to a multiple of 8)")
+    _unfollowed("linear_int8")
+    x, sx = _dense(rows.codes), rows.scales.contiguous()
+    y = torch.empty((m, n), dtype=torch.float16, device=dev)
+    with _lib.on(dev):
+        status = _lib.lib().s3d_linear_int8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), None if bias is None else bias.data_ptr(),
+                                            y.data_ptr(), m, n, k, int(bool(gelu)), _lib.stream(dev))
+    _lib.check(status, "s3d_linear_int8")
+    return y
+
+
+def mlp_int8(rows, weight1, bias1, weight2, bias2):
+    """linear_int8(quantize_rows(linear_int8(rows, weight1, bias1, gelu=True)), weight2, bias2) as one call.  Both widths are multiples
+    of 16 up to 8192; biases as for linear_int8, either may be None."""
+    _check_rows("rows", rows)
+    m, c = rows.codes.shape
+    dev = rows.codes.device
+    w1, s1, bias1 = _layer_operands("weight1", weight1, bias1, c, dev)
+    hidden = w1.shape[0]
+    w2, s2, bias2 = _layer_operands("weight2", weight2, bias2, hidden, dev)
+    if w2.shape[0] != c or any(w == 0 or w % 16 or w > _MOST_HIDDEN for w in (c, hidden)):
+        raise ValueError(f"an MLP from {c} over {hidden} to {w2.shape[0]} channels (back to as many, multiples of 16 up to {_MOST_HIDDEN})")
+    _unfollowed("mlp_int8")
+    x, sx = _dense(rows.codes), rows.scales.contiguous()
+    y = torch.empty((m, c), dtype=torch.float16, device=dev)
+    lib = _lib.lib()
+    with _lib.on(dev):
+        ws_bytes = lib.s3d_mlp_int8_workspace_bytes(m, c, hidden)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        status = lib.s3d_mlp_int8(x.data_ptr(), sx.data_ptr(), w1.data_ptr(), s1.data_ptr(), None if bias1 is None else bias1.data_ptr(), w2.data_ptr(),
+                                  s2.data_ptr(), None if bias2 is None else bias2.data_ptr(), y.data_ptr(), m, c, hidden, workspace.data_ptr(), ws_bytes,
+                                  _lib.stream(dev))
+    _lib.check(status, "s3d_mlp_int8")
+    return y
+
+
+# ---- checkpoints -------------------------------------------------------------------------------------------------------------
+
+def _check_width(name, width):
+    if width == 0 or width % 16 or width > _MOST_WIDTH:
+        raise ValueError(f"{name} of {width} channels (a multiple of 16, at most {_MOST_WIDTH})")
+
+
+def _kept_buffer(m, k, device):
+    return torch.empty(m * k + m * (k // 16), dtype=torch.uint8, device=device)
+
+
+def keep_rows(x):
+    """uint8 [17 N C / 16]: fp16 rows [N,C] in eight bits, in groups of sixteen numbers: codes int8 [N,C], then a byte with the scale of
+    every group (s3d_keep_rows has the form).  C is a multiple of 16, at most 16384.  x is taken as its data."""
+    _check("x", x, (torch.float16,), (None, None))
+    m, k = x.shape
+    _check_width("rows", k)
+    _unfollowed("keep_rows")
+    x = _dense(x.detach())
+    kept = _kept_buffer(m, k, x.device)
+    with _lib.on(x.device):
+        status = _lib.lib().s3d_keep_rows(x.data_ptr(), kept.data_ptr(), m, k, _lib.stream(x.device))
+    _lib.check(status, "s3d_keep_rows")
+    return kept
+
+
+def kept_values(kept, channels):
+    """fp16 [N,channels]: what kept rows stand for, exactly."""
+    _check("kept", kept, (torch.uint8,), (None,))
+    _check_width("rows", channels)
+    m, rest = divmod(kept.numel(), channels + channels // 16)
+    if rest:
+        raise ValueError(f"{kept.numel()} bytes are no whole number of rows of {channels} channels")
+    _unfollowed("kept_values")
+    kept = _dense(kept)
+    out = torch.empty((m, channels), dtype=torch.float16, device=kept.device)
+    with _lib.on(kept.device):
+        status = _lib.lib().s3d_kept_values(kept.data_ptr(), out.data_ptr(), m, channels, _lib.stream(kept.device))
+    _lib.check(status, "s3d_kept_values")
+    return out
+
+
+def _copies(weight, bias, turned):
+    """(weight, its transpose or None, bias or None) in fp16, as the kernels read them."""
+    done = _half_copies(weight, bias, turned) if weight.dtype == torch.float32 and (bias is None or bias.dtype == torch.float32) else None
+    if done is None:
+        half = _dense(weight.to(torch.float16))
+        done = half, half.t().contiguous() if turned else None, None if bias is None else _dense(bias.to(torch.float16))
+    return done
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+
+def _rows_like(t, dtype):
+    """A gradient that came in, as the kernels read it."""
+    return _dense(t if t.dtype == dtype else t.to(dtype))
+
+
+def _parameter_gradients(dtypes, needs, shapes, rows, device):
+    """(type, gradients or None): one type for all of them, fp32 if any of those wanted is; zeros where there are no rows."""
+    wanted = [d for d, need in zip(dtypes, needs) if need]
+    dtype = torch.float32 if not wanted or torch.float32 in wanted else torch.float16
+    make = torch.empty if rows else torch.zeros
+    return dtype, [make(shape, dtype=dtype, device=device) if need else None for shape, need in zip(shapes, needs)]
+
+
+class _KeptLinear(Function):
+    """graph: whether one is recorded; without it nothing is kept."""
+
+    @staticmethod
+    def forward(ctx, graph, x, weight, bias):
+        need_x, need_weight, _ = (graph and need for need in ctx.needs_input_grad[1:])
+        (m, k), n, dev = x.shape, weight.shape[0], x.device
+        half, turned, half_bias = _copies(weight, bias, need_x)
+        rows = _dense(x)
+        y = torch.empty((m, n), dtype=torch.float16, device=dev)
+        kept = _kept_buffer(m, k, dev) if need_weight else None
+        if m:
+            with _lib.on(dev):
+                status = _lib.lib().s3d_kept_linear(rows.data_ptr(), half.data_ptr(), _ptr(half_bias), y.data_ptr(), _ptr(kept), m, n, k, _lib.stream(dev))
+            _lib.check(status, "s3d_kept_linear")
+        ctx.save_for_backward(kept, turned)
+        ctx.shapes, ctx.dtypes = (m, n, k), [None if p is None else p.dtype for p in (weight, bias)]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        kept, turned = ctx.saved_tensors
+        (m, n, k), dev, needs = ctx.shapes, dy.device, ctx.needs_input_grad[1:]
+        dx = torch.empty((m, k), dtype=torch.float16, device=dev) if needs[0] else None
+        dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((n, k), (n,)), m, dev)
+        if m and (dx is not None or any(g is not None for g in grads)):
+            dy = _rows_like(dy, torch.float16)
+            lib = _lib.lib()
+            with _lib.on(dev):
+                ws_bytes = lib.s3d_kept_linear_grad_workspace_bytes(m, n, k)
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+                status = lib.s3d_kept_linear_grad(dy.data_ptr(), _ptr(turned), _ptr(kept), _ptr(dx), *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, n, k,
+                                                  workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+            _lib.check(status, "s3d_kept_linear_grad")
+        return (None, dx, *(g if g is None or g.dtype == d else g.to(d) for g, d in zip(grads, ctx.dtypes)))
+
+
+class _KeptMlp(Function):
+    @staticmethod
+    def forward(ctx, graph, x, weight1, bias1, weight2, bias2):
+        needs = [graph and need for need in ctx.needs_input_grad[1:]]
+        (m, c), hidden, dev = x.shape, weight1.shape[0], x.device
+        behind = any(needs[:3])
+        half1, turned1, half_bias1 = _copies(weight1, bias1, needs[0])
+        half2, turned2, half_bias2 = _copies(weight2, bias2, behind)
+        rows = _dense(x)
+        y = torch.empty((m, c), dtype=torch.float16, device=dev)
+        kept_x = _kept_buffer(m, c, dev) if needs[1] else None
+        kept_h = _kept_buffer(m, hidden, dev) if behind or needs[3] else None
+        if m:
+            lib = _lib.lib()
+            with _lib.on(dev):
+                ws_bytes = lib.s3d_kept_mlp_workspace_bytes(m, c, hidden)
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+                status = lib.s3d_kept_mlp(rows.data_ptr(), half1.data_ptr(), _ptr(half_bias1), half2.data_ptr(), _ptr(half_bias2), y.data_ptr(), _ptr(kept_x),
+                                          _ptr(kept_h), m, c, hidden, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+            _lib.check(status, "s3d_kept_mlp")
+        ctx.save_for_backward(kept_x, kept_h, turned1, turned2)
+        ctx.shapes = (m, c, hidden)
+        ctx.dtypes = [None if p is None else p.dtype for p in (weight1, bias1, weight2, bias2)]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        kept_x, kept_h, turned1, turned2 = ctx.saved_tensors
+        needs, (m, c, hidden), dev = ctx.needs_input_grad[1:], ctx.shapes, dy.device
+        dx = torch.empty((m, c), dtype=torch.float16, device=dev) if needs[0] else None
+        dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((hidden, c), (hidden,), (c, hidden), (c,)), m, dev)
+        if m:
+            dy = _rows_like(dy, torch.float16)
+            lib = _lib.lib()
+            with _lib.on(dev):
+                ws_bytes = lib.s3d_kept_mlp_grad_workspace_bytes(m, c, hidden)
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+                status = lib.s3d_kept_mlp_grad(dy.data_ptr(), _ptr(turned1), _ptr(turned2), _ptr(kept_x), _ptr(kept_h), _ptr(dx), *(_ptr(g) for g in grads),
+                                               _DTYPE_CODE[dtype], m, c, hidden, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+            _lib.check(status, "s3d_kept_mlp_grad")
+        return (None, dx, *(g if g is None or g.dtype == d else g.to(d) for g, d in zip(grads, ctx.dtypes)))
+
+
+def _check_layer(name, weight, bias, k, dev):
+    _check(name, weight, tuple(_DTYPE_CODE), (None, k), dev)
+    if bias is not None:
+        _check(f"the bias of {name}", bias, tuple(_DTYPE_CODE), (weight.shape[0],), dev)
+    _check_width(f"{name}: rows", k)
+    _check_width(f"{name}: results", weight.shape[0])
+
+
+def _no_followers(what):
+    if followed():
+        raise RuntimeError(f"{what} does not run under a transform, a forward-mode derivative, a dispatch mode or a tracer")
+
+
+def checkpointed_linear(x, weight, bias=None):
+    """F.linear(x, weight, bias) in fp16 for fp16 rows [N,in] and parameters in fp16 or fp32, which keeps x for its backward in eight
+    bits: 1.0625 bytes a number in place of two.  y and the gradient of x are those of the layer in fp16; the gradients of the parameters come in
+    their own type, weight's from what was kept.  Widths are multiples of 16 up to 16384.  Gradients of gradients are refused."""
+    _check("x", x, (torch.float16,), (None, None))
+    _check_layer("weight", weight, bias, x.shape[1], x.device)
+    _no_followers("checkpointed_linear")
+    return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias)
+
+
+def checkpointed_mlp(x, weight1, bias1, weight2, bias2):
+    """F.linear(F.gelu(F.linear(x, weight1, bias1)), weight2, bias2) in fp16 for fp16 rows [N,C] and parameters in fp16 or fp32, which keeps
+    x and the hidden layer's rows in front of GELU in eight bits: for a hidden layer of 4 C channels 5.3 C bytes a row, where x and the hidden layer on both
+    sides of GELU are 18 C.  The gradients go by what was kept.  Widths are multiples of 16 up to 16384, biases may be None.  Gradients of gradients
+    are refused."""
+    _check("x", x, (torch.float16,), (None, None))
+    c = x.shape[1]
+    _check_layer("weight1", weight1, bias1, c, x.device)
+    _check_layer("weight2", weight2, bias2, weight1.shape[0], x.device)
+    if weight2.shape[0] != c:
+        raise ValueError(f"an MLP from {c} to {weight2.shape[0]} channels (back to as many)")
+    _no_followers("checkpointed_mlp")
+    return _KeptMlp.apply(torch.is_grad_enabled(), x, weight1, bias1, weight2, bias2)

@@ -1,0 +1,81 @@
+"""What the dense layers in eight bits refuse, without a device: shapes, types and null pointers at the C entry points, CPU tensors and
+other objects at the Python ones; and the statement of the kept form that the GPU tests use."""
+import ctypes
+
+import pytest
+import torch
+
+from eight_bit_reference import keep, kept, kept_scales
+from swin3d_amd import eight_bits
+from swin3d_amd.eight_bits import Int8Rows
+
+
+def _refused(lib, status, text):
+    assert status < 0 and text in lib.s3d_last_error_string().decode()
+
+
+def test_c_entry_points_refuse(hip_lib):
+    lib, one = hip_lib, ctypes.c_void_p(16)
+    for n, c in ((-1, 48), (4, 0), (4, 6), (4, 8196), (1 << 31, 48)):
+        _refused(lib, lib.s3d_add_norm_int8(one, None, 0, one, one, 1e-5, 0, None, one, one, n, c, None), "s3d_add_norm_int8: N=")
+        _refused(lib, lib.s3d_quantize_rows(one, 0, one, one, n, c, None), "s3d_quantize_rows: N=")
+        _refused(lib, lib.s3d_int8_values(one, one, one, 0, n, c, None), "s3d_int8_values: N=")
+    _refused(lib, lib.s3d_add_norm_int8(one, one, 7, one, one, 1e-5, 0, None, one, one, 4, 48, None), "residual_dtype 7")
+    _refused(lib, lib.s3d_quantize_rows(one, 2, one, one, 4, 48, None), "dtype 2")
+    _refused(lib, lib.s3d_int8_values(one, one, one, 2, 4, 48, None), "dtype 2")
+    _refused(lib, lib.s3d_add_norm_int8(None, None, 0, one, one, 1e-5, 0, None, one, one, 4, 48, None), "null")
+    _refused(lib, lib.s3d_quantize_rows(one, 0, None, one, 4, 48, None), "null")
+    _refused(lib, lib.s3d_int8_values(one, None, one, 0, 4, 48, None), "null")
+    for m, n, k in ((-1, 16, 16), (4, 12, 16), (4, 16, 24), (4, 0, 16), (4, 16, 0), (4, 16, 65552), (1 << 31, 16, 16)):
+        _refused(lib, lib.s3d_linear_int8(one, one, one, one, None, one, m, n, k, 0, None), "s3d_linear_int8: M=")
+    _refused(lib, lib.s3d_linear_int8(one, None, one, one, None, one, 4, 16, 16, 0, None), "null")
+    for m, c, hidden in ((-1, 16, 16), (4, 24, 16), (4, 16, 24), (4, 16, 8208), (4, 8208, 16)):
+        _refused(lib, lib.s3d_mlp_int8(*[one] * 9, m, c, hidden, one, 1 << 30, None), "s3d_mlp_int8: M=")
+        assert lib.s3d_mlp_int8_workspace_bytes(m, c, hidden) == 0
+    _refused(lib, lib.s3d_mlp_int8(*[one] * 9, 4, 16, 16, one, 16, None), "workspace 16 B")
+    for m, k in ((-1, 16), (4, 24), (4, 0), (4, 16400)):
+        _refused(lib, lib.s3d_keep_rows(one, one, m, k, None), "s3d_keep_rows: M=")
+        _refused(lib, lib.s3d_kept_values(one, one, m, k, None), "s3d_kept_values: M=")
+        assert lib.s3d_kept_bytes(m, k) == 0
+    assert lib.s3d_kept_bytes(100, 48) == 100 * 51
+    for m, n, k in ((0, 16, 16), (4, 24, 16), (4, 16, 24), (4, 16, 16400), (4, 16400, 16)):
+        _refused(lib, lib.s3d_kept_linear(one, one, None, one, one, m, n, k, None), "s3d_kept_linear: M=")
+        _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, m, n, k, one, 1 << 30, None), "s3d_kept_linear_grad: M=")
+        _refused(lib, lib.s3d_kept_mlp(*[one] * 8, m, k, n, one, 1 << 30, None), "s3d_kept_mlp: M=")
+        _refused(lib, lib.s3d_kept_mlp_grad(*[one] * 10, 0, m, k, n, one, 1 << 30, None), "s3d_kept_mlp_grad: M=")
+    _refused(lib, lib.s3d_kept_linear(one, None, None, one, one, 4, 16, 16, None), "null")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, None, one, one, one, 0, 4, 16, 16, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_linear_grad(one, None, one, one, one, one, 0, 4, 16, 16, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 2, 4, 16, 16, one, 1 << 30, None), "grad_dtype 2")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, 4, 16, 16, one, 8, None), "workspace 8 B")
+    _refused(lib, lib.s3d_kept_mlp(one, one, None, None, None, one, one, one, 4, 16, 16, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_mlp(*[one] * 8, 4, 16, 16, one, 8, None), "workspace 8 B")
+    _refused(lib, lib.s3d_kept_mlp_grad(one, one, one, one, None, one, one, one, one, one, 0, 4, 16, 16, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_mlp_grad(*[one] * 10, 3, 4, 16, 16, one, 1 << 30, None), "grad_dtype 3")
+    _refused(lib, lib.s3d_kept_mlp_grad(*[one] * 10, 0, 4, 16, 16, None, 1 << 30, None), "workspace 0 B")
+
+
+def test_cpu_tensors_and_other_objects_are_refused():
+    x, norm = torch.randn(4, 48), torch.nn.LayerNorm(48)
+    rows = Int8Rows(torch.zeros(4, 48, dtype=torch.int8), torch.zeros(4))
+    for bad in (lambda: eight_bits.add_norm_int8(x, None, norm), lambda: eight_bits.quantize_rows(x), lambda: eight_bits.linear_int8(rows, rows),
+                lambda: eight_bits.mlp_int8(rows, rows, None, rows, None), lambda: rows.values(), lambda: eight_bits.keep_rows(x.half()),
+                lambda: eight_bits.kept_values(torch.zeros(51, dtype=torch.uint8), 48), lambda: eight_bits.checkpointed_linear(x.half(), x),
+                lambda: eight_bits.checkpointed_mlp(x.half(), x, None, x.t(), None), lambda: eight_bits.quantize_rows([1.0]),
+                lambda: eight_bits.linear_int8([1], rows), lambda: eight_bits.add_norm_int8(None, None, norm)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_statement_of_the_kept_form():
+    """Scales ascend, have four bits, and codes times scales are fp16 numbers."""
+    scales = kept_scales()
+    assert scales[0] == 0 and scales[1] == 1 and all(a < b for a, b in zip(scales, scales[1:]))
+    assert all(s >> max(0, s.bit_length() - 4) << max(0, s.bit_length() - 4) == s for s in scales)
+    assert scales[249] == 576 << 24 and 127 * scales[248] < 65504 << 24 <= 127 * scales[249]
+    x = torch.randn(200, 64) * torch.exp(5 * torch.randn(200, 1))
+    x = x.clamp(-65504, 65504).half()
+    x[0], x[1, :32], x[1, 16] = 65504.0, 0.0, 6e-8
+    values = kept(x)
+    assert torch.equal(values.half().double(), values) and int(keep(x)[0].abs().max()) == 127
+    assert torch.equal(values[1, :17], x[1, :17].double())
