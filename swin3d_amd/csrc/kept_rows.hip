@@ -30,12 +30,12 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(const _Float16 *__restri
     }
 }
 
-// x Phi(x) as the forward has it
+// GELU as the kernels have it that take its derivative too
 __device__ __forceinline__ half8 gelu_of(const half8 &v)
 {
     half8 u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = static_cast<_Float16>(gelu(v[e]));
+    for (int e = 0; e < 8; ++e) u[e] = to_half(gelu_and_slope(v[e]).value);
     return u;
 }
 
@@ -103,17 +103,16 @@ MlpLayers mlp_layers(int64_t M, int32_t C, int32_t hidden)
 {
     return {{{nullptr, nullptr, nullptr, nullptr, M, C, hidden, 0, 1.0f}, {nullptr, nullptr, nullptr, nullptr, M, hidden, C, 0, 1.0f}}};
 }
-// x', h', GELU(h') and dh, and the parts of the weights' gradients
+// x', GELU(h') and dh, and the parts of the weights' gradients
 struct MlpPlaces {
-    size_t x, hidden, active, dhidden, parts, total;
+    size_t x, active, dhidden, parts, total;
 };
 MlpPlaces mlp_places(int64_t M, int32_t C, int32_t hidden)
 {
     MlpPlaces p{};
     const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
     const MlpLayers layers = mlp_layers(M, C, hidden);
-    p.hidden = align_up(2 * codes_bytes(M, C), 256);
-    p.active = p.hidden + wide;
+    p.active = align_up(2 * codes_bytes(M, C), 256);
     p.dhidden = p.active + wide;
     p.parts = p.dhidden + wide;
     p.total = p.parts + linear_grads_bytes(layers.of, 2);
@@ -190,7 +189,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
 {
-    return fits(M, hidden, C) ? 2 * align_up(2 * codes_bytes(M, hidden), 256) : 0;
+    return fits(M, hidden, C) ? align_up(2 * codes_bytes(M, hidden), 256) : 0;      // (GELU of the hidden layer)
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *y,
@@ -199,20 +198,19 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x
 {
     if (!fits(M, hidden, C)) return bad_shape("s3d_kept_mlp", M, hidden, C);
     if (!x || !w1 || !w2 || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_mlp: null device pointer");
-    const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
-    if (!workspace || workspace_bytes < 2 * wide)
-        return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), 2 * wide);
-    char *h = static_cast<char *>(workspace), *active = h + wide;
+    const size_t need = s3d_kept_mlp_workspace_bytes(M, C, hidden);
+    if (!workspace || workspace_bytes < need)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), need);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (kept_mlp_pays(M, C, hidden, false)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, M, C, hidden}, false, s);
     if (kept_x)
         if (int rc = keep(x, kept_x, M, C, s)) return rc;
-    LinearArgs first{x, w1, b1, h, M, hidden, C, false};
-    first.in_order = true;
-    first.gelu_out = active;
+    LinearArgs first{x, w1, b1, workspace, M, hidden, C, false};
+    first.keep = true;
+    first.kept = kept_h;
+    first.gelu_out = workspace;
     if (int rc = launch_linear(first, s)) return rc;
-    if (kept_h)
-        if (int rc = keep(h, kept_h, M, hidden, s)) return rc;
-    return launch_linear({active, w2, b2, y, M, C, hidden, false}, s);
+    return launch_linear({workspace, w2, b2, y, M, C, hidden, false}, s);
 }
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_grad_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
@@ -236,16 +234,24 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
         return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);
     char *base = static_cast<char *>(workspace), *active = base + p.active, *dhidden = base + p.dhidden;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (behind || dw2)
-        if (int rc = values(kept_h, behind ? base + p.hidden : nullptr, dw2 ? active : nullptr, M, hidden, s)) return rc;
+    if (!behind && dw2)
+        if (int rc = values(kept_h, nullptr, active, M, hidden, s)) return rc;
     LinearGrad grads[2];
     int num = 0;
     if (dw2 || db2) grads[num++] = LinearGrad{dy, dw2 ? active : dy, dw2, db2, M, C, dw2 ? hidden : 16, 0, 1.0f};
     if (behind) {
-        LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false, base + p.hidden};
-        if (int rc = launch_linear(a, s)) return rc;
-        if (dx)
-            if (int rc = launch_linear({dhidden, w1_t, nullptr, dx, M, C, hidden, false}, s)) return rc;
+        if (dx && kept_mlp_pays(M, C, hidden, true)) {
+            const KeptMlp a{dy, w2_t, nullptr, w1_t, nullptr, dx, nullptr, const_cast<void *>(kept_h), dhidden, active, M, C, hidden};
+            if (int rc = launch_kept_mlp(a, true, s)) return rc;
+        } else {
+            LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false};
+            a.kept_grad = true;
+            a.kept = kept_h;
+            a.gelu_out = active;
+            if (int rc = launch_linear(a, s)) return rc;
+            if (dx)
+                if (int rc = launch_linear({dhidden, w1_t, nullptr, dx, M, C, hidden, false}, s)) return rc;
+        }
     }
     if (dw1 || db1) {
         if (dw1)

@@ -14,6 +14,11 @@ struct LinearArgs {
     const void *gelu_at = nullptr;   // [M,N] fp16: the rows, rounded, are gradients behind a GELU of these, and y those before it
     bool in_order = false;           // a number's K products are added up one after the other, whatever the tile
     void *gelu_out = nullptr;        // [M,N] fp16: GELU of y's rounded rows, beside them (in_order; without gelu and gelu_at)
+    // Rows in eight bits (rows8.h; without gelu, gelu_at and in_order, N a multiple of 16).  keep: in place of y the rounded rows go there
+    // (unless kept is null) and GELU of them to gelu_out.  kept_grad: the rows are gradients behind a GELU of what is kept there, y those
+    // before it, and gelu_out GELU of what is kept.
+    bool keep = false, kept_grad = false;
+    const void *kept = nullptr;
 };
 
 int launch_linear(const LinearArgs &a, hipStream_t stream);
@@ -41,6 +46,19 @@ struct LinearInt8 {
 int launch_linear_int8(const LinearInt8 &l, hipStream_t stream);
 // Rows of fp32 or fp16 in eight bits with a scale each (norm_int8.hip)
 int launch_quantize_rows(const void *x, int32_t dtype, int8_t *codes, float *scales, int64_t N, int32_t C, hipStream_t stream);
+
+// Both layers of an MLP in training that keeps its inputs in eight bits, in one kernel each way (kept_mlp.hip)
+struct KeptMlp {
+    const void *x, *w1, *b1, *w2, *b2;   // forward: [M,C], [hidden,C], [hidden] or null, [C,hidden], [C] or null; fp16
+    void *y;                             // [M,C]
+    void *kept_x, *kept_h;               // written by the forward unless null; kept_h is read by the backward
+    void *dh, *active;                   // backward, [M,hidden] fp16: the hidden layer's gradients, and GELU of what is kept
+    int64_t M;
+    int32_t C, hidden;
+};
+bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden, bool backward);
+// the backward's x is dy, w1 and w2 are w2 and w1 transposed, y is dx; no biases
+int launch_kept_mlp(const KeptMlp &a, bool backward, hipStream_t stream);
 
 // A layer's weight and bias gradients (linear_grad.hip): dw = dy^T x, db = the column sums of dy; the first `scaled` rows of
 // the weight (and numbers of the bias) are parameters times `scale`

@@ -15,6 +15,7 @@
 #include "attn_kernels.h"
 #include "dense.h"
 #include "linear.h"
+#include "rows8.h"
 
 #include <type_traits>
 
@@ -25,38 +26,12 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 64;        // numbers of K staged at a time
 static_assert(kChunk / 8 == kPieces, "pieces of eight numbers");
 
-// The derivative of x Phi(x): Phi(x) + x phi(x), in fp32.  With Phi(-u) = phi(u) M(u), M the ratio of Mills, that is
-// phi(u) (u - M(u)) with the sign of x, and 1 more for x above 0, u = |x|: u - M(u) by the polynomial of degree 12 that fits
-// phi(u) (u - M(u)) best over [0, 5.8], 8.7e-9 off at most, up to 5, where phi is still large enough to hold its relative error, and by
-// a line from there on, where u - M(u) is close to one.  Over all fp16 numbers the error is the rounding of fp32, 9.2e-8 at most
-// (1.47e-7 with erff and the exponential apart).  Where the derivative is small and negative it is a relative 1.4e-4 at most from -3 to
-// -5, 1.0e-3 to -8 and 6.5e-3 to -13 (1.7e-3, 3.3e-2 and 2.1e-2, since 1 + erf cancels there; with the polynomial alone 3e-2 at -5.8, and beyond -6.8
-// the other sign).  Infinities and NaN as the sum of
-// the two terms has them: NaN.  A third of the instructions less: 199,327 rows of 48 to 192, us, 52.6 -> 41.5, 49,682 of 96 to 384
-// 33.4 -> 27.0, 12,421 of 192 to 768 24.2 -> 19.0, with their rows alone 18, 15 and 12.
-__device__ __forceinline__ float gelu_slope(float x)
-{
-    const float u = fabsf(x), c = fminf(u, 5.0f), phi = __builtin_amdgcn_exp2f(fmaf(u * u, -0.7213475204f, -1.325748064f));
-    float q = fmaf(-1.467262933e-07f, c, 4.019878816e-06f);
-    q = fmaf(q, c, -4.986505519e-05f);
-    q = fmaf(q, c, 3.754729696e-04f);
-    q = fmaf(q, c, -1.954356674e-03f);
-    q = fmaf(q, c, 7.658625022e-03f);
-    q = fmaf(q, c, -2.421350777e-02f);
-    q = fmaf(q, c, 6.534569710e-02f);
-    q = fmaf(q, c, -1.560686380e-01f);
-    q = fmaf(q, c, 3.331732452e-01f);
-    q = fmaf(q, c, -6.266347766e-01f);
-    q = fmaf(q, c, 1.999998808e+00f);
-    q = fmaf(q, c, -1.253314137e+00f);
-    q = fmaf(u - c, 1.025f, q);
-    return fmaf(__builtin_copysignf(phi, x), q, 0.5f + __builtin_copysignf(0.5f, x));
-}
-
 // x Phi(x) of a training forward, as torch has it: by the math library's erff, in this order of operations
 __device__ __forceinline__ float gelu_erf(float x) { return (x * 0.5f) * (1.0f + erff(x * 0.70710678f)); }
 
-enum class Behind { kNothing, kGelu, kGeluGrad, kGeluBeside };
+// The last two are of layers that keep rows in eight bits (kept_rows.hip), in `gelu_at`'s place: kKeep leaves the rows' codes and GELU of
+// the rows, rounded, in `gelu_out`; kKeptGrad multiplies by GELU's slope at what was kept, in fp32, and leaves GELU of that in `gelu_out`.
+enum class Behind { kNothing, kGelu, kGeluGrad, kGeluBeside, kKeep, kKeptGrad };
 
 // WM x WN wavefronts of TM x TN products of 32 x 32
 template <int WM, int WN, int TM, int TN> struct Tile {
@@ -147,7 +122,8 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
             for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
         // the chunk is there, and nobody reads the other buffer any more
         auto meet = [&]() {
-            if (inside) loads_done<TM * 2 * TN * (kBehind == Behind::kGeluBeside ? 2 : 1)>();
+            if (inside && kBehind == Behind::kKeep && gelu_at) loads_done<TM * 2 * TN * 3>();
+            else if (inside) loads_done<TM * 2 * TN * (kBehind == Behind::kGeluBeside || kBehind == Behind::kKeptGrad ? 2 : 1)>();
             else loads_done<0>();
             inside = false;
             workgroup_barrier();
@@ -179,6 +155,21 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
                     at[i][t] = *reinterpret_cast<const half8 *>(gelu_at + static_cast<int64_t>(r) * N + min(n0 + wave_n + e % kRowPieces * 8, N - 8));
                 }
         }
+        uint8_t *const kept = const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(gelu_at)), *const kept_scales = kept + static_cast<int64_t>(M) * N;
+        uint4 codes[TM][TN];
+        uint32_t scales[TM][TN][2];
+        if constexpr (kBehind == Behind::kKeptGrad) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int64_t r = min(m0 + wave_m + i * 32 + r32, M - 1);
+                    const int n = n0 + wave_n + j * 32;
+                    codes[i][j] = *reinterpret_cast<const uint4 *>(kept + r * N + min(n + 16 * half, N - 16));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) scales[i][j][k] = kept_scales[r * (N / kKeptGroup) + min(n / kKeptGroup + k, N / kKeptGroup - 1)];
+                }
+        }
         const int next = tile + step;
         if (next < end) {
             aim(next / tiles_n * L::kM, next % tiles_n * L::kN);
@@ -192,6 +183,49 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
         _Float16 *out = reinterpret_cast<_Float16 *>(smem + buffer * L::kStage) + wave * (32 * L::kPitch);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
+            if constexpr (kBehind == Behind::kKeptGrad) {
+                uint2 active[TN][4];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    // words 2 g + half of the row's eight, where the lanes hold four neighbouring ones each
+                    const auto a02 = __builtin_amdgcn_permlane32_swap(codes[i][j].x, codes[i][j].y, false, false);
+                    const auto a13 = __builtin_amdgcn_permlane32_swap(codes[i][j].z, codes[i][j].w, false, false);
+                    const uint32_t word[4] = {a02[0], a13[0], a02[1], a13[1]};
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float s = kept_scale(scales[i][j][g / 2]);
+                        const float at_codes[4] = {code_of<0>(word[g]), code_of<1>(word[g]), code_of<2>(word[g]), code_of<3>(word[g])};
+                        half4 o, u;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const Active v = gelu_and_slope(at_codes[e] * s);
+                            o[e] = to_half(acc[i][j][4 * g + e] * v.slope);
+                            u[e] = to_half(v.value);
+                        }
+                        *reinterpret_cast<half4 *>(out + r32 * L::kPitch + j * 32 + 8 * g + 4 * half) = o;
+                        active[j][g] = __builtin_bit_cast(uint2, u);
+                    }
+                }
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    wave_fence();
+#pragma unroll
+                    for (int t = 0; t < 2 * TN; ++t) {
+                        const int e = t * 64 + lane, r = e / kRowPieces, n = e % kRowPieces * 8;
+                        const half8 v = *reinterpret_cast<const half8 *>(out + r * L::kPitch + n);
+                        if (inside || (m0 + wave_m + i * 32 + r < M && n0 + wave_n + n < N))
+                            *reinterpret_cast<half8 *>((which ? gelu_out : y) + static_cast<int64_t>(m0 + wave_m + i * 32 + r) * N + n0 + wave_n + n) = v;
+                    }
+                    wave_fence();
+                    if (which == 0) {
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) *reinterpret_cast<uint2 *>(out + r32 * L::kPitch + j * 32 + 8 * g + 4 * half) = active[j][g];
+                    }
+                }
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -214,6 +248,20 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
                 }
                 const int64_t to = static_cast<int64_t>(m0 + wave_m + i * 32 + r) * N + n0 + wave_n + n;
                 const bool there = inside || (m0 + wave_m + i * 32 + r < M && n0 + wave_n + n < N);
+                if constexpr (kBehind == Behind::kKeep) {
+                    // (a row's neighbouring pieces, which make a group, are in neighbouring lanes)
+                    const uint32_t own = largest_bits(v), other = __builtin_amdgcn_update_dpp(0u, own, 0xb1, 0xf, 0xf, true);
+                    if (gelu_at) {
+                        const uint32_t byte = kept_byte(max(own, other));
+                        const uint2 c = kept_codes(v, Divisor(byte));
+                        if (there) *reinterpret_cast<uint2 *>(kept + to) = c;
+                        if (there && n % kKeptGroup == 0) kept_scales[to / kKeptGroup] = static_cast<uint8_t>(byte);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = to_half(gelu(static_cast<float>(v[k])));
+                    if (there) *reinterpret_cast<half8 *>(gelu_out + to) = v;
+                    continue;
+                }
                 if (there) *reinterpret_cast<half8 *>(y + to) = v;
                 if constexpr (kBehind == Behind::kGeluBeside) {
 #pragma unroll
@@ -234,14 +282,15 @@ int launch(const LinearArgs &a, hipStream_t stream)
     if (tiles > (1 << 30)) return fail(S3D_ERR_BAD_SHAPE, "s3d_linear: M = %lld rows", (long long)a.M);
     auto kernel = a.gelu ? linear_kernel<L, Behind::kGelu> : linear_kernel<L, Behind::kNothing>;
     if constexpr (L::kTN < 3) kernel = a.gelu_at ? linear_kernel<L, Behind::kGeluGrad> : kernel;
-    if constexpr (L::kTM == 1 && L::kTN == 1) kernel = a.gelu_out ? linear_kernel<L, Behind::kGeluBeside> : kernel;
+    if constexpr (L::kTN < 3) kernel = a.keep ? linear_kernel<L, Behind::kKeep> : a.kept_grad ? linear_kernel<L, Behind::kKeptGrad> : kernel;
+    if constexpr (L::kTM == 1 && L::kTN == 1) kernel = a.gelu_out && !a.keep && !a.kept_grad ? linear_kernel<L, Behind::kGeluBeside> : kernel;
     // as many workgroups as fit the chip (by LDS), or one a tile
     constexpr int kPerCu = 160 * 1024 / L::kLds < 2 ? 1 : 160 * 1024 / L::kLds < 4 ? 160 * 1024 / L::kLds : 4;
     const int64_t slots = static_cast<int64_t>(kPerCu) * device_cus();
     const dim3 grid(static_cast<unsigned>(ceil_div(tiles < slots ? tiles : slots, 8) * 8));
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, static_cast<const _Float16 *>(a.x), static_cast<const _Float16 *>(a.w),
-                       static_cast<const _Float16 *>(a.bias), static_cast<_Float16 *>(a.y), static_cast<const _Float16 *>(a.gelu_at),
-                       static_cast<_Float16 *>(a.gelu_out), static_cast<int>(a.M), a.N, a.K, tiles_n, static_cast<int>(tiles));
+                       static_cast<const _Float16 *>(a.bias), static_cast<_Float16 *>(a.y),
+                       static_cast<const _Float16 *>(a.keep || a.kept_grad ? a.kept : a.gelu_at), static_cast<_Float16 *>(a.gelu_out), static_cast<int>(a.M), a.N, a.K, tiles_n, static_cast<int>(tiles));
     S3D_HIP_CHECK(hipGetLastError());
     return S3D_OK;
 }
@@ -360,7 +409,8 @@ int launch_linear(const LinearArgs &a, hipStream_t stream)
     // 640 0.86 to 1.00; 520 at K = 320 4.8 / 5.8, at 640 5.9 / 6.2, at 2560 23.0 / 13.9; 588 at K = 1536 10.4 / 10.0; 980 at 2560 23.7 / 19.4,
     // at 640 6.3 / 8.0; 1880 at 2560 27.0 / 35.4.
     const int64_t thin = ceil_div(a.M, 32) * ((a.N + 31) / 32);
-    if (!a.gelu_at && !a.in_order && (thin <= 256 || (thin <= 512 && a.K >= 192) || (thin <= 1024 && a.K >= 2048))) return launch_thin(a, stream);
+    const bool eight_bits = a.keep || a.kept_grad;
+    if (!a.gelu_at && !a.in_order && !eight_bits && (thin <= 256 || (thin <= 512 && a.K >= 192) || (thin <= 1024 && a.K >= 2048))) return launch_thin(a, stream);
     // Tiles of 64 x 64 as long as larger ones would leave CUs without work: up to 576 of them, with GELU or its derivative, whose
     // instructions more wavefronts hide, up to 1024 (768 and 576 to 192, 64 x 64 / 128 x 64, us, by number: 288 6.7 / 7.0, 576 8.8 / 8.5,
     // 720 9.4 / 9.1, 864 11.8 / 9.6; with GELU 585 9.6 / 10.6).  With GELU's derivative and up to 384 channels until there
@@ -378,12 +428,12 @@ int launch_linear(const LinearArgs &a, hipStream_t stream)
     // 49,682 of 96 to 384 30.8 / 34.9 / 26.5, 12,421 of 192 to 768 25.8 / 23.3 / 17.1, 3,105 of 384 to 1536 19.9 / 14.9 / 12.6;
     // 6,250 of 96 11.2 / 7.4.
     const int64_t small = ceil_div(a.M, 64) * ((a.N + 63) / 64);
-    const bool heavy = a.gelu || a.gelu_at;
-    if (a.gelu_out || small < (heavy ? 1024 : 576) || (a.gelu_at && a.K <= 384 && small <= 6144)) return launch<Tile<2, 2, 1, 1>>(a, stream);
+    const bool heavy = a.gelu || a.gelu_at || eight_bits;
+    if ((a.gelu_out && !eight_bits) || small < (heavy ? 1024 : 576) || (a.gelu_at && a.K <= 384 && small <= 6144)) return launch<Tile<2, 2, 1, 1>>(a, stream);
     auto padded = [&](int width) { return (a.N + width - 1) / width * width; };
     auto count = [&](int width) { return ceil_div(a.M, 128) * (padded(width) / width); };
     const int least = padded(64);
-    if (padded(192) == least && count(192) >= 512 && !a.gelu_at && (!a.gelu || a.N <= 192)) return launch<Tile<2, 2, 2, 3>>(a, stream);
+    if (padded(192) == least && count(192) >= 512 && !a.gelu_at && !eight_bits && (!a.gelu || a.N <= 192)) return launch<Tile<2, 2, 2, 3>>(a, stream);
     if (padded(128) == least && ((count(128) >= (heavy ? 448 : 384) && count(128) <= 512) || count(128) >= 640)) return launch<Tile<2, 2, 2, 2>>(a, stream);
     return launch<Tile<2, 2, 2, 1>>(a, stream);
 }

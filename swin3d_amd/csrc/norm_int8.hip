@@ -135,10 +135,17 @@ __global__ __launch_bounds__(kThreads) void rows_int8_kernel(RowArgs a)
         const float a_max = finite ? __uint_as_float(most) : 0.0f;
         // (127 / a_max stays finite, and a product with it exact enough, for the smallest rows too)
         const float lift = a_max < 0x1p-100f ? 0x1p100f : 1.0f, inverse = a_max > 0.0f ? 127.0f / (a_max * lift) : 0.0f;
+        const float reciprocal = HALF && a_max > 0.0f ? 1.0f / a_max : 0.0f;
 #pragma unroll
         for (int i = 0; i < FOURS; ++i) {
             if (lane + i * G >= fours) continue;
-            auto code = [&](float x) { return __float_as_uint(fmaf(finite ? x * lift : 0.0f, inverse, 12582912.0f)); };
+            // Rows of fp16 numbers have ties: where the largest is 127 / 2^n of another number, one number in some twenty lies between two
+            // codes exactly.  Their quotient 127 x / a_max is the correctly rounded one (127 x is exact), so that these go to even.
+            auto code = [&](float x) {
+                if (!HALF) return __float_as_uint(fmaf(finite ? x * lift : 0.0f, inverse, 12582912.0f));
+                const float q = x * inverse;
+                return __float_as_uint(finite ? fmaf(fmaf(-q, a_max, 127.0f * x), reciprocal, q) + 12582912.0f : 0.0f);
+            };
             *reinterpret_cast<uint32_t *>(a.codes + row * C + 4 * (lane + i * G)) = four_bytes(code(v[i].x), code(v[i].y), code(v[i].z), code(v[i].w));
         }
         if (lane == 0) a.scales[row] = finite ? a_max / 127.0f : __builtin_nanf("");

@@ -23,14 +23,14 @@ __device__ __forceinline__ float kept_scale(uint32_t byte)
     return byte == kKeptNaN ? __builtin_nanf("") : __uint_as_float(byte << 20) * 0x1p105f;
 }
 
-// The byte of a group's largest size, given as an fp32 number (that is an fp16 number) by its bits.  Truncated, a / 127 is the scale
-// or the one below, also where the quotient's rounding crosses one; 127 times a scale is exact.
+// The byte of a group's largest size, by its fp16 bits.  Truncated, a / 127 is the scale or the one below, also where the quotient's
+// rounding crosses one; 127 times a scale is exact.
 __device__ __forceinline__ uint32_t kept_byte(uint32_t largest)
 {
-    if (largest >= 0x7f800000u) return kKeptNaN;
-    const float a = __uint_as_float(largest);
+    const float a = __builtin_bit_cast(_Float16, static_cast<uint16_t>(largest));
     const uint32_t byte = __float_as_uint(a * (1.0f / 127.0f) * 0x1p-105f) >> 20;
-    return byte + (127.0f * kept_scale(byte) < a ? 1 : 0);
+    const uint32_t up = byte + (127.0f * (__uint_as_float(byte << 20) * 0x1p105f) < a ? 1 : 0);
+    return largest >= 0x7c00u ? kKeptNaN : up;
 }
 
 // What turns numbers into codes of a scale
@@ -38,20 +38,19 @@ struct Divisor {
     float scale, inverse, most;
     __device__ __forceinline__ explicit Divisor(uint32_t byte)
     {
-        scale = kept_scale(byte);
         const bool none = byte == 0 || byte == kKeptNaN;
-        scale = none ? 0.0f : scale;
-        inverse = none ? 0.0f : 1.0f / scale;
-        most = byte >= 249 ? 113.0f : 127.0f;      // (114 times the largest scale, 576, would round to infinity in fp16)
+        scale = none ? 0.0f : kept_scale(byte);
+        inverse = none ? 0.0f : __builtin_amdgcn_rcpf(scale);
+        most = none ? 0.0f : byte >= 249 ? 113.0f : 127.0f;      // (114 times the largest scale, 576, would round to infinity in fp16)
     }
     // x / scale to the nearest whole number, ties to even, as the low byte of the result.  The correction makes the quotient the
-    // correctly rounded one, without which 2,214 of the 3,981,084 pairs of an fp16 number and a scale that reaches it get the other
-    // neighbour of a tie.
+    // correctly rounded one, with a reciprocal that is a unit off too; without it 2,214 of the 3,981,084 pairs of an fp16 number and a scale
+    // that reaches it get the other neighbour of a tie.
     __device__ __forceinline__ uint32_t code(float x) const
     {
         float q = x * inverse;
         q = fmaf(fmaf(-q, scale, x), inverse, q);
-        q = fminf(fmaxf(q, -most), most);
+        q = __builtin_amdgcn_fmed3f(q, -most, most);
         return __float_as_uint(q + 12582912.0f);      // 1.5 x 2^23: whole numbers lie one unit apart
     }
 };
@@ -80,19 +79,43 @@ __device__ __forceinline__ half8 kept_numbers(uint2 codes, uint32_t byte)
     return v;
 }
 
-// the largest size among eight numbers, as fp32 bits, which order infinity and NaN behind all others
+// the largest size among numbers, as fp16 bits, which order infinity and NaN behind all others
+typedef uint16_t bits2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(bits2, a), __builtin_bit_cast(bits2, b)));
+}
 __device__ __forceinline__ uint32_t largest_bits(const half8 &v)
 {
-    uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(static_cast<float>(v[e])) & 0x7fffffffu);
-    return most;
+    const uint4 w = __builtin_bit_cast(uint4, v);
+    const uint32_t pair = larger_pair(larger_pair(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), larger_pair(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+    return max(pair >> 16, pair & 0xffffu);
 }
 
+__device__ __forceinline__ uint32_t kept_codes(const half4 &v, const Divisor &d) { return four_bytes(d.code(v[0]), d.code(v[1]), d.code(v[2]), d.code(v[3])); }
 __device__ __forceinline__ uint2 kept_codes(const half8 &v, const Divisor &d)
 {
     return make_uint2(four_bytes(d.code(v[0]), d.code(v[1]), d.code(v[2]), d.code(v[3])),
                       four_bytes(d.code(v[4]), d.code(v[5]), d.code(v[6]), d.code(v[7])));
+}
+
+// fp32 first, then fp16: where the compiler makes one instruction of the last operation and the conversion, as it does in some kernels and
+// not in others, a number in some 70,000 is the other neighbour of a tie
+__device__ __forceinline__ _Float16 to_half(float v)
+{
+    asm volatile("" : "+v"(v));
+    return static_cast<_Float16>(v);
+}
+
+// x Phi(x) and its derivative at once, of numbers that are finite or NaN: in the terms of gelu_slope, u phi(u) M(u) is what x Phi(x)
+// is below the larger of x and 0.
+struct Active {
+    float value, slope;
+};
+__device__ __forceinline__ Active gelu_and_slope(float x)
+{
+    const GeluTail t = gelu_tail(x);
+    return {fmaf(-t.u * t.phi, t.u - t.q, fmaxf(x, 0.0f)), fmaf(__builtin_copysignf(t.phi, x), t.q, 0.5f + __builtin_copysignf(0.5f, x))};
 }
 
 }  // namespace s3d
