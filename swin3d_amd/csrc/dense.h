@@ -83,6 +83,11 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const void *from)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0", "memory");
 }
+// ... from `base`, the same for all lanes, and a lane's offset in bytes
+__device__ __forceinline__ void load_to_lds_from(uint32_t to, const void *base, uint32_t offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "m0", "memory");
+}
 #pragma clang diagnostic pop
 // ... all but the kBehind instructions issued last
 template <int kBehind> __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kBehind) : "memory"); }

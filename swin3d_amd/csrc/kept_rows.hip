@@ -50,6 +50,88 @@ __global__ __launch_bounds__(kThreads) void kept_values_kernel(const uint8_t *__
     }
 }
 
+// Parameters as the products read them: fp16 copies of those in fp32, and transposed ones of weights.  Tiles of 64 x 64 that turn in LDS;
+// a bias is a matrix of one row.
+constexpr int kSquare = 64, kMostCopies = 4;
+struct Copies {
+    const void *from[kMostCopies];
+    _Float16 *to[kMostCopies], *turned[kMostCopies];      // either may be null
+    int rows[kMostCopies], cols[kMostCopies], first[kMostCopies];
+    bool half[kMostCopies];
+    int num, blocks;
+
+    // adds `from` where anything is wanted of it; what the products read of it
+    const void *add(const void *array, int32_t dtype, int32_t r, int32_t c, void *copy, void *transposed)
+    {
+        const bool as_is = dtype == S3D_DTYPE_F16;
+        if (!array || (as_is && !transposed)) return array;
+        from[num] = array;
+        to[num] = as_is ? nullptr : static_cast<_Float16 *>(copy);
+        turned[num] = static_cast<_Float16 *>(transposed);
+        rows[num] = r;
+        cols[num] = c;
+        half[num] = as_is;
+        first[num++] = blocks;
+        blocks += (r + kSquare - 1) / kSquare * ((c + kSquare - 1) / kSquare);
+        return as_is ? array : copy;
+    }
+};
+
+__global__ __launch_bounds__(kThreads) void copies_kernel(Copies a)
+{
+    __shared__ __align__(16) _Float16 tile_s[kSquare][kSquare + 4];
+    int which = 0;
+#pragma unroll
+    for (int i = 1; i < kMostCopies; ++i) which = i < a.num && static_cast<int>(blockIdx.x) >= a.first[i] ? i : which;
+    const void *from = a.from[0];
+    _Float16 *to = a.to[0], *turned = a.turned[0];
+    int rows = a.rows[0], cols = a.cols[0], first = a.first[0];
+    bool half = a.half[0];
+#pragma unroll
+    for (int i = 1; i < kMostCopies; ++i) {
+        if (which != i) continue;
+        from = a.from[i]; to = a.to[i]; turned = a.turned[i]; rows = a.rows[i]; cols = a.cols[i]; first = a.first[i]; half = a.half[i];
+    }
+    const int across = (cols + kSquare - 1) / kSquare, tile = static_cast<int>(blockIdx.x) - first, r0 = tile / across * kSquare, c0 = tile % across * kSquare;
+    const int four = threadIdx.x % 16 * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = threadIdx.x / 16 + 16 * i;
+        if (r0 + r >= rows || c0 + four >= cols) continue;
+        const int64_t at = static_cast<int64_t>(r0 + r) * cols + c0 + four;
+        half4 v;
+        if (half) {
+            v = *reinterpret_cast<const half4 *>(static_cast<const _Float16 *>(from) + at);
+        } else {
+            const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(from) + at);
+            v = half4{static_cast<_Float16>(f.x), static_cast<_Float16>(f.y), static_cast<_Float16>(f.z), static_cast<_Float16>(f.w)};
+        }
+        if (to) *reinterpret_cast<half4 *>(to + at) = v;
+        *reinterpret_cast<half4 *>(&tile_s[r][four]) = v;
+    }
+    if (!turned) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = threadIdx.x / 16 + 16 * i;
+        if (c0 + c >= cols || r0 + four >= rows) continue;
+        const half4 v = {tile_s[four][c], tile_s[four + 1][c], tile_s[four + 2][c], tile_s[four + 3][c]};
+        *reinterpret_cast<half4 *>(turned + static_cast<int64_t>(c0 + c) * rows + r0 + four) = v;
+    }
+}
+
+int launch_copies(const Copies &a, hipStream_t stream)
+{
+    if (a.blocks == 0) return S3D_OK;
+    hipLaunchKernelGGL(copies_kernel, dim3(a.blocks), dim3(kThreads), 0, stream, a);
+    S3D_HIP_CHECK(hipGetLastError());
+    return S3D_OK;
+}
+
+bool is_dtype(int32_t d) { return d == S3D_DTYPE_F32 || d == S3D_DTYPE_F16; }
+// room for the copies of a weight and a bias
+size_t copies_bytes(int32_t N, int32_t K) { return align_up(2 * static_cast<size_t>(N) * K, 256) + align_up(2 * static_cast<size_t>(N), 256); }
+
 dim3 grid_of(int64_t threads)
 {
     const int64_t blocks = ceil_div(threads, kThreads);
@@ -83,39 +165,26 @@ int values(const void *kept, void *out, void *active, int64_t M, int32_t K, hipS
     return S3D_OK;
 }
 
-// x' and the parts of the weight's gradient
-struct LinearPlaces {
-    size_t x, parts, total;
-};
-LinearPlaces linear_places(int64_t M, int32_t N, int32_t K)
+size_t linear_parts_bytes(int64_t M, int32_t N, int32_t K, bool kept)
 {
-    LinearPlaces p{};
-    const LinearGrad g{nullptr, nullptr, nullptr, nullptr, M, N, K, 0, 1.0f};
-    p.parts = align_up(2 * codes_bytes(M, K), 256);
-    p.total = p.parts + linear_grads_bytes(&g, 1);
-    return p;
+    // (for the bias alone the other operand is any rows of 16 channels)
+    LinearGrad g{nullptr, nullptr, nullptr, nullptr, M, N, K, 0, 1.0f}, bias{nullptr, nullptr, nullptr, nullptr, M, N, 16, 0, 1.0f};
+    g.kept = kept;
+    const size_t all = kept_grads_bytes(&g, 1), some = kept_grads_bytes(&bias, 1);
+    return all > some ? all : some;
 }
 
-struct MlpLayers {
-    LinearGrad of[2];      // fc2, fc1
-};
-MlpLayers mlp_layers(int64_t M, int32_t C, int32_t hidden)
-{
-    return {{{nullptr, nullptr, nullptr, nullptr, M, C, hidden, 0, 1.0f}, {nullptr, nullptr, nullptr, nullptr, M, hidden, C, 0, 1.0f}}};
-}
-// x', GELU(h') and dh, and the parts of the weights' gradients
+// GELU(h') and dh, and the parts of the weights' gradients
 struct MlpPlaces {
-    size_t x, active, dhidden, parts, total;
+    size_t active, dhidden, parts, total;
 };
 MlpPlaces mlp_places(int64_t M, int32_t C, int32_t hidden)
 {
     MlpPlaces p{};
     const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
-    const MlpLayers layers = mlp_layers(M, C, hidden);
-    p.active = align_up(2 * codes_bytes(M, C), 256);
     p.dhidden = p.active + wide;
     p.parts = p.dhidden + wide;
-    p.total = p.parts + linear_grads_bytes(layers.of, 2);
+    p.total = p.parts + linear_parts_bytes(M, C, hidden, false) + linear_parts_bytes(M, hidden, C, true);
     return p;
 }
 
@@ -145,12 +214,28 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_values(const void
     return values(kept, out, nullptr, M, K, static_cast<hipStream_t>(stream));
 }
 
-extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void *x, const void *w, const void *bias, void *y, void *kept, int64_t M, int32_t N,
-                                                                      int32_t K, void *stream)
+extern "C" __attribute__((visibility("default"))) size_t s3d_kept_linear_workspace_bytes(int32_t N, int32_t K)
+{
+    return fits(1, N, K) ? copies_bytes(N, K) : 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void *x, const void *w, int32_t w_dtype, const void *bias, int32_t bias_dtype,
+                                                                      void *y, void *kept, void *w_t, int64_t M, int32_t N, int32_t K, void *workspace,
+                                                                      size_t workspace_bytes, void *stream)
 {
     if (!fits(M, N, K)) return bad_shape("s3d_kept_linear", M, N, K);
+    if (!is_dtype(w_dtype) || (bias && !is_dtype(bias_dtype)))
+        return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_linear: dtypes %d, %d (0 = fp32, 1 = fp16)", w_dtype, bias_dtype);
     if (!x || !w || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear: null device pointer");
+    const size_t need = copies_bytes(N, K);
+    if (!workspace || workspace_bytes < need)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_linear: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), need);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    char *base = static_cast<char *>(workspace);
+    Copies copies{};
+    w = copies.add(w, w_dtype, N, K, base, w_t);
+    bias = copies.add(bias, bias_dtype, 1, N, base + align_up(2 * static_cast<size_t>(N) * K, 256), nullptr);
+    if (int rc = launch_copies(copies, s)) return rc;
     if (kept)
         if (int rc = keep(x, kept, M, K, s)) return rc;
     return launch_linear({x, w, bias, y, M, N, K, false}, s);
@@ -158,7 +243,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_kept_linear_grad_workspace_bytes(int64_t M, int32_t N, int32_t K)
 {
-    return fits(M, N, K) ? linear_places(M, N, K).total : 0;
+    return fits(M, N, K) ? linear_parts_bytes(M, N, K, true) : 0;
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void *dx, void *dw, void *db,
@@ -169,48 +254,59 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const
     if (grad_dtype != S3D_DTYPE_F32 && grad_dtype != S3D_DTYPE_F16)
         return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_linear_grad: grad_dtype %d (0 = fp32, 1 = fp16)", grad_dtype);
     if (!dy || (dx && !w_t) || (dw && !kept)) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear_grad: null device pointer");
-    const LinearPlaces p = linear_places(M, N, K);
-    if (!workspace || workspace_bytes < p.total)
-        return fail(S3D_ERR_WORKSPACE, "s3d_kept_linear_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);
-    char *base = static_cast<char *>(workspace);
+    const size_t need = linear_parts_bytes(M, N, K, true);
+    if (!workspace || workspace_bytes < need)
+        return fail(S3D_ERR_WORKSPACE, "s3d_kept_linear_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), need);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dx)
         if (int rc = launch_linear({dy, w_t, nullptr, dx, M, K, N, false}, s)) return rc;
     if (!dw && !db) return S3D_OK;
-    if (dw) {
-        if (int rc = values(kept, base + p.x, nullptr, M, K, s)) return rc;
-    }
-    // (for the bias alone the other operand is any rows)
-    LinearGrad g{dy, dw ? base + p.x : dy, dw, db, M, N, dw ? K : 16, 0, 1.0f};
-    float *parts = reinterpret_cast<float *>(base + p.parts);
-    if (int rc = launch_linear_grad_parts(&g, 1, &parts, s)) return rc;
+    LinearGrad g{dy, dw ? kept : dy, dw, db, M, N, dw ? K : 16, 0, 1.0f};
+    g.kept = dw;
+    float *parts = static_cast<float *>(workspace);
+    if (int rc = launch_kept_grad_parts(&g, 1, &parts, s)) return rc;
     return launch_linear_grad_sums(&g, 1, nullptr, grad_dtype, s);
 }
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
 {
-    return fits(M, hidden, C) ? align_up(2 * codes_bytes(M, hidden), 256) : 0;      // (GELU of the hidden layer)
+    if (!fits(M, hidden, C)) return 0;
+    // copies of the parameters, and GELU of the hidden layer where the layers are two products
+    return copies_bytes(hidden, C) + copies_bytes(C, hidden) + (kept_mlp_pays(M, C, hidden, false) ? 0 : align_up(2 * codes_bytes(M, hidden), 256));
 }
 
-extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *y,
-                                                                   void *kept_x, void *kept_h, int64_t M, int32_t C, int32_t hidden, void *workspace,
-                                                                   size_t workspace_bytes, void *stream)
+extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2,
+                                                                   const int32_t *dtypes, void *y, void *kept_x, void *kept_h, void *w1_t, void *w2_t,
+                                                                   int64_t M, int32_t C, int32_t hidden, void *workspace, size_t workspace_bytes,
+                                                                   void *stream)
 {
     if (!fits(M, hidden, C)) return bad_shape("s3d_kept_mlp", M, hidden, C);
-    if (!x || !w1 || !w2 || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_mlp: null device pointer");
+    if (!x || !w1 || !w2 || !y || !dtypes) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_mlp: null pointer");
+    for (int i = 0; i < 4; ++i)
+        if (!is_dtype(dtypes[i])) return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_mlp: dtype %d (0 = fp32, 1 = fp16)", dtypes[i]);
     const size_t need = s3d_kept_mlp_workspace_bytes(M, C, hidden);
     if (!workspace || workspace_bytes < need)
         return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), need);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    char *base = static_cast<char *>(workspace);
+    const size_t whole = align_up(2 * static_cast<size_t>(hidden) * C, 256);
+    Copies copies{};
+    w1 = copies.add(w1, dtypes[0], hidden, C, base, w1_t);
+    b1 = copies.add(b1, dtypes[1], 1, hidden, base + whole, nullptr);
+    base += copies_bytes(hidden, C);
+    w2 = copies.add(w2, dtypes[2], C, hidden, base, w2_t);
+    b2 = copies.add(b2, dtypes[3], 1, C, base + whole, nullptr);
+    base += copies_bytes(C, hidden);
+    if (int rc = launch_copies(copies, s)) return rc;
     if (kept_mlp_pays(M, C, hidden, false)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, M, C, hidden}, false, s);
     if (kept_x)
         if (int rc = keep(x, kept_x, M, C, s)) return rc;
-    LinearArgs first{x, w1, b1, workspace, M, hidden, C, false};
+    LinearArgs first{x, w1, b1, base, M, hidden, C, false};
     first.keep = true;
     first.kept = kept_h;
-    first.gelu_out = workspace;
+    first.gelu_out = base;
     if (int rc = launch_linear(first, s)) return rc;
-    return launch_linear({workspace, w2, b2, y, M, C, hidden, false}, s);
+    return launch_linear({base, w2, b2, y, M, C, hidden, false}, s);
 }
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_grad_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
@@ -254,12 +350,11 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
         }
     }
     if (dw1 || db1) {
-        if (dw1)
-            if (int rc = values(kept_x, base + p.x, nullptr, M, C, s)) return rc;
-        grads[num++] = LinearGrad{dhidden, dw1 ? static_cast<const void *>(base + p.x) : dhidden, dw1, db1, M, hidden, dw1 ? C : 16, 0, 1.0f};
+        grads[num] = LinearGrad{dhidden, dw1 ? kept_x : dhidden, dw1, db1, M, hidden, dw1 ? C : 16, 0, 1.0f};
+        grads[num++].kept = dw1;
     }
     if (num == 0) return S3D_OK;
     float *parts = reinterpret_cast<float *>(base + p.parts);
-    if (int rc = launch_linear_grad_parts(grads, num, &parts, s)) return rc;
+    if (int rc = launch_kept_grad_parts(grads, num, &parts, s)) return rc;
     return launch_linear_grad_sums(grads, num, nullptr, grad_dtype, s);
 }

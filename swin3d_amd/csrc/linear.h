@@ -70,6 +70,7 @@ struct LinearGrad {
     float scale;
     const float *parts = nullptr;   // where launch_linear_grad_parts has put them, and how many
     int32_t splits = 0;
+    bool kept = false;              // x in eight bits (rows8.h), for launch_kept_grad_parts
 };
 
 constexpr int kMostLinearGrads = 4;
@@ -77,6 +78,10 @@ constexpr int kMostLinearGrads = 4;
 size_t linear_grads_bytes(const LinearGrad *grads, int num);
 // the parts of `num` layers of as many rows, to *parts and on, which is moved behind them
 int launch_linear_grad_parts(LinearGrad *grads, int num, float **parts, hipStream_t stream);
+
+// The same for layers that keep their input in eight bits, and of an MLP's hidden layer in fp16 (kept_grad.hip); N and K multiples of 16
+size_t kept_grads_bytes(const LinearGrad *grads, int num);
+int launch_kept_grad_parts(LinearGrad *grads, int num, float **parts, hipStream_t stream);
 
 // The gradients of (sum, y) = (x + residual, LayerNorm(x + residual)) (layernorm.hip), those of the norm's parameters in parts
 struct NormGrad {

@@ -453,11 +453,13 @@ int launch_linear_int8(const LinearInt8 &l, hipStream_t stream)
     // 7.4 / 8.3, 882 6.4 / 5.9, 1440 12.5 / 11.6, 1470 8.6 / 7.9, 1565 19.2 / 19.4, 3130 26.5 / 20.2); then 128 rows by 128 columns where that pads
     // N no more than 64 (128 x 64 / so: 20,000 rows, 640 to 1920 50.9 / 46.2; 100,000, 256 to 384 36.1 / 32.7; 60,000, 192 to 768 with GELU
     // 45.2 / 43.0; 37,499, 320 to 1280 with GELU 53.7 / 52.8), by 96 likewise (60,000, 192 to 576 24.8 / 22.5; 100,000, 384 to 96 16.2 / 13.6;
-    // 6,250, 320 to 960 7.9 / 7.5), else by 64.
-    if (ceil_div(l.M, 64) * ((l.N + 63) / 64) < 1024) return launch<Tile<2, 2, 1, 1>>(a, l.gelu, stream);
+    // 6,250, 320 to 960 7.9 / 7.5), else by 64.  With GELU, whose instructions more wavefronts hide, up to 320 channels 64 x 64 up to 6144 of them
+    // (12,421, 192 to 768 11.7 / 11.1; 49,682, 96 to 384 17.3 / 16.6), and never 96 (18.9, 13.2).
+    const int64_t small = ceil_div(l.M, 64) * ((l.N + 63) / 64);
+    if (small < 1024 || (l.gelu && l.K <= 320 && small <= 6144)) return launch<Tile<2, 2, 1, 1>>(a, l.gelu, stream);
     auto padded = [&](int width) { return (l.N + width - 1) / width * width; };
     if (padded(128) == padded(64) && ceil_div(l.M, 128) * (padded(128) / 128) >= 640) return launch<Tile<2, 2, 2, 2>>(a, l.gelu, stream);
-    if (padded(96) <= padded(64)) return launch<Tile<4, 1, 1, 3>>(a, l.gelu, stream);
+    if (padded(96) <= padded(64) && !l.gelu) return launch<Tile<4, 1, 1, 3>>(a, l.gelu, stream);
     return launch<Tile<4, 1, 1, 2>>(a, l.gelu, stream);
 }
 

@@ -63,19 +63,23 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t 
 // code i of four, as a number
 template <int I> __device__ __forceinline__ float code_of(uint32_t four) { return static_cast<float>(static_cast<int>(four << (24 - 8 * I)) >> 24); }
 
-// eight codes times their scale: exact
+// Eight codes times their scale, in fp16 arithmetic, in which every step is exact: a byte below 0x64 is 1024 + it, less 1152 the code (whose
+// sign bit was turned), and that times the scale is an fp16 number.
 __device__ __forceinline__ half8 kept_numbers(uint2 codes, uint32_t byte)
 {
-    const float s = kept_scale(byte);
+    const _Float16 s = static_cast<_Float16>(kept_scale(byte)), offset = static_cast<_Float16>(1152.0f);
+    const half2 scale = {s, s}, offsets = {offset, offset};
     half8 v;
-    v[0] = static_cast<_Float16>(code_of<0>(codes.x) * s);
-    v[1] = static_cast<_Float16>(code_of<1>(codes.x) * s);
-    v[2] = static_cast<_Float16>(code_of<2>(codes.x) * s);
-    v[3] = static_cast<_Float16>(code_of<3>(codes.x) * s);
-    v[4] = static_cast<_Float16>(code_of<0>(codes.y) * s);
-    v[5] = static_cast<_Float16>(code_of<1>(codes.y) * s);
-    v[6] = static_cast<_Float16>(code_of<2>(codes.y) * s);
-    v[7] = static_cast<_Float16>(code_of<3>(codes.y) * s);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const uint32_t four = (w ? codes.y : codes.x) ^ 0x80808080u;
+        const half2 lo = (__builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, four, 0x04010400u)) - offsets) * scale;
+        const half2 hi = (__builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, four, 0x04030402u)) - offsets) * scale;
+        v[4 * w] = lo[0];
+        v[4 * w + 1] = lo[1];
+        v[4 * w + 2] = hi[0];
+        v[4 * w + 3] = hi[1];
+    }
     return v;
 }
 

@@ -19,6 +19,8 @@ their group's largest number off at most, and an eighth of that more where a sca
 All take dense CUDA (HIP) tensors, enqueue on torch's current stream of their device and do not wait.  What is wrong with an argument
 raises ValueError, CPU tensors included.
 """
+import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -26,7 +28,6 @@ import torch.nn as nn
 from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
-from .linear_grad import _half_copies
 from .swin_blocks import followed
 
 _DTYPE_CODE = {torch.float32: _lib.S3D_DTYPE_F32, torch.float16: _lib.S3D_DTYPE_F16}
@@ -47,7 +48,7 @@ class Int8Rows(NamedTuple):
         if c == 0 or c % 4 or c > _MOST_CHANNELS:
             raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
         dev = self.codes.device
-        codes, scales = _dense(self.codes), self.scales.contiguous()
+        codes, scales = _dense(self.codes), _dense(self.scales)
         out = torch.empty((n, c), dtype=dtype, device=dev)
         with _lib.on(dev):
             status = _lib.lib().s3d_int8_values(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), _DTYPE_CODE[dtype], n, c, _lib.stream(dev))
@@ -62,25 +63,38 @@ def _dense(t):
 
 
 def _check(name, t, dtypes, shape, device=None):
-    """t is a plain tensor on the GPU (on `device`) of one of the dtypes and of `shape`, in which None stands for any size."""
+    """t is a tensor on the GPU (on `device`) of one of the dtypes and of `shape`, in which None stands for any size."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-    if not t.is_cuda or t.dtype not in dtypes or t.dim() != len(shape) or any(s is not None and s != got for s, got in zip(shape, t.shape)) \
+    sizes = t.shape
+    if not t.is_cuda or t.dtype not in dtypes or len(sizes) != len(shape) or any(s is not None and s != got for s, got in zip(shape, sizes)) \
             or (device is not None and t.device != device):
-        sizes = ",".join("any" if s is None else str(s) for s in shape)
+        wanted = ",".join("any" if s is None else str(s) for s in shape)
         kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         where = "on a CUDA (HIP) device" if device is None else f"on {device}"
-        raise ValueError(f"{name} must be {kinds} [{sizes}] {where}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.dim() and t.shape[0] > 0x7fffffff:
-        raise ValueError(f"{name} has {t.shape[0]} rows (at most 2^31 - 1)")
+        raise ValueError(f"{name} must be {kinds} [{wanted}] {where}, got {t.dtype} {tuple(sizes)} on {t.device}")
+    if sizes[0] > 0x7fffffff:
+        raise ValueError(f"{name} has {sizes[0]} rows (at most 2^31 - 1)")
 
 
 def _check_rows(name, rows, device=None):
     if not isinstance(rows, tuple) or len(rows) != 2:
         raise ValueError(f"{name} must be Int8Rows, got {type(rows).__name__}")
     codes, scales = rows
-    _check(f"{name}.codes", codes, (torch.int8,), (None, None), device)
-    _check(f"{name}.scales", scales, (torch.float32,), (codes.shape[0],), codes.device)
+    _check(f"{name}.codes", codes, _INT8, _ANY_ROWS, device)
+    _check(f"{name}.scales", scales, _FP32, (codes.shape[0],), codes.device)
+
+
+_INT8, _FP32, _FP16, _EITHER = (torch.int8,), (torch.float32,), (torch.float16,), (torch.float16, torch.float32)
+_ANY_ROWS = (None, None)
+
+
+def _ready(dev, *tensors):
+    """All of them (None aside) are plain, dense and 16-byte aligned on `dev`: nothing about them has to be looked at or copied but shapes and types."""
+    return all(t is None or (type(t) in _PLAIN and t.device == dev and t.is_contiguous() and t.data_ptr() % 16 == 0) for t in tensors)
+
+
+_PLAIN = (torch.Tensor, nn.Parameter)
 
 
 def _unfollowed(what, *tensors):
@@ -102,7 +116,7 @@ def add_norm_int8(x, residual, norm, inplace=False):
     inplace    write the sum back into x instead of a new tensor
     C is a multiple of 4 and at most 8192.  A row with a number that is not finite stands for NaN.  No autograd.
     """
-    _check("x", x, (torch.float32,), (None, None))
+    _check("x", x, _FP32, _ANY_ROWS)
     n, c = x.shape
     dev = x.device
     if c == 0 or c % 4 or c > _MOST_CHANNELS:
@@ -112,10 +126,10 @@ def add_norm_int8(x, residual, norm, inplace=False):
         raise ValueError(f"norm must be a LayerNorm or RMSNorm over the {c} channels, got {norm}")
     weight, bias = norm.weight, None if rms else norm.bias
     for name, p in (("norm.weight", weight), ("norm.bias", bias)):
-        if p is not None:
+        if p is not None and not (p.dtype is torch.float32 and p.device == dev and p.dim() == 1):      # (its size is normalized_shape's)
             _check(name, p, (torch.float32, torch.float16, torch.bfloat16, torch.float64), (c,), dev)
     if residual is not None:
-        _check("residual", residual, tuple(_DTYPE_CODE), (n, c), dev)
+        _check("residual", residual, _EITHER, (n, c), dev)
     _unfollowed("add_norm_int8", x, residual, weight, bias)
     if inplace and residual is not None and not (x.is_contiguous() and x.data_ptr() % 16 == 0):
         raise ValueError("x must be contiguous and 16-byte aligned to be written in place")
@@ -126,7 +140,7 @@ def add_norm_int8(x, residual, norm, inplace=False):
         residual = _dense(residual)
         res_ptr, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]
         summed = x if inplace else torch.empty((n, c), dtype=torch.float32, device=dev)
-    gamma, beta = (None if p is None else _dense(p.detach().float()) for p in (weight, bias))
+    gamma, beta = (None if p is None else _dense(p if p.dtype is torch.float32 else p.detach().float()) for p in (weight, bias))
     rows = _empty_rows(n, c, dev)
     with _lib.on(dev):
         status = _lib.lib().s3d_add_norm_int8(
@@ -139,7 +153,7 @@ def add_norm_int8(x, residual, norm, inplace=False):
 def quantize_rows(x):
     """Int8Rows of fp16 or fp32 rows [N,C]: the input of a layer, or a weight [out,in].  scale = max |row| / 127, code = row / scale to the
     nearest, ties to even.  C is a multiple of 4 and at most 8192.  No autograd: x is taken as its data."""
-    _check("x", x, tuple(_DTYPE_CODE), (None, None))
+    _check("x", x, _EITHER, _ANY_ROWS)
     n, c = x.shape
     if c == 0 or c % 4 or c > _MOST_CHANNELS:
         raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
@@ -156,13 +170,32 @@ def quantize_rows(x):
 def _layer_operands(name, weight, bias, k, dev):
     """(codes, scales, bias or None) of a layer of k inputs, as the kernels read them."""
     _check_rows(name, weight, dev)
-    n = weight.codes.shape[0]
-    if weight.codes.shape[1] != k:
-        raise ValueError(f"{name} takes {weight.codes.shape[1]} channels, the rows have {k}")
+    codes, scales = weight
+    n = codes.shape[0]
+    if codes.shape[1] != k:
+        raise ValueError(f"{name} takes {codes.shape[1]} channels, the rows have {k}")
     if bias is not None:
         _check(f"the bias of {name}", bias, (torch.float32, torch.float16), (n,), dev)
         bias = _dense(bias.detach().float())
-    return _dense(weight.codes), _dense(weight.scales), bias
+    return _dense(codes), _dense(scales), bias
+
+
+def _product_operands(rows, weight, bias):
+    """(x, its scales, w, its scales, bias or None, rows, inputs, outputs, device), as the kernels read them."""
+    if isinstance(rows, tuple) and isinstance(weight, tuple) and len(rows) == len(weight) == 2:
+        (x, sx), (w, sw) = rows, weight
+        # (the usual operands: each is looked at once)
+        if isinstance(x, torch.Tensor) and x.is_cuda and _ready(x.device, x, sx, w, sw, bias) and x.dtype is w.dtype is torch.int8 \
+                and sx.dtype is sw.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32):
+            a, b = x.shape, w.shape
+            if len(a) == len(b) == 2 and a[1] == b[1] and sx.shape == a[:1] and sw.shape == b[:1] and (bias is None or bias.shape == b[:1]) \
+                    and a[0] <= 0x7fffffff:
+                return x, sx, w, sw, bias, a[0], a[1], b[0], x.device
+    _check_rows("rows", rows)
+    m, k = rows[0].shape
+    dev = rows[0].device
+    w, sw, bias = _layer_operands("weight", weight, bias, k, dev)
+    return _dense(rows[0]), _dense(rows[1]), w, sw, bias, m, k, w.shape[0], dev
 
 
 def linear_int8(rows, weight, bias=None, gelu=False):
@@ -173,15 +206,10 @@ def linear_int8(rows, weight, bias=None, gelu=False):
     bias     fp32 or fp16 [out], or None
     The sums are exact, scales, bias and GELU fp32, with one rounding at the end.  in is a multiple of 16 up to 65536, out of 8.  No autograd.
     """
-    _check_rows("rows", rows)
-    m, k = rows.codes.shape
-    dev = rows.codes.device
-    w, sw, bias = _layer_operands("weight", weight, bias, k, dev)
-    n = w.shape[0]
+    x, sx, w, sw, bias, m, k, n, dev = _product_operands(rows, weight, bias)
     if k == 0 or k % 16 or k > _MOST_SUMMED or n == 0 or n % 8:
         raise ValueError(f"a layer from {k} to {n} channels (from a multiple of 16 up to {_MOST_SUMMED}, to a multiple of 8)")
     _unfollowed("linear_int8")
-    x, sx = _dense(rows.codes), rows.scales.contiguous()
     y = torch.empty((m, n), dtype=torch.float16, device=dev)
     with _lib.on(dev):
         status = _lib.lib().s3d_linear_int8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -193,16 +221,11 @@ def linear_int8(rows, weight, bias=None, gelu=False):
 def mlp_int8(rows, weight1, bias1, weight2, bias2):
     """linear_int8(quantize_rows(linear_int8(rows, weight1, bias1, gelu=True)), weight2, bias2) as one call.  Both widths are multiples
     of 16 up to 8192; biases as for linear_int8, either may be None."""
-    _check_rows("rows", rows)
-    m, c = rows.codes.shape
-    dev = rows.codes.device
-    w1, s1, bias1 = _layer_operands("weight1", weight1, bias1, c, dev)
-    hidden = w1.shape[0]
+    x, sx, w1, s1, bias1, m, c, hidden, dev = _product_operands(rows, weight1, bias1)
     w2, s2, bias2 = _layer_operands("weight2", weight2, bias2, hidden, dev)
     if w2.shape[0] != c or any(w == 0 or w % 16 or w > _MOST_HIDDEN for w in (c, hidden)):
         raise ValueError(f"an MLP from {c} over {hidden} to {w2.shape[0]} channels (back to as many, multiples of 16 up to {_MOST_HIDDEN})")
     _unfollowed("mlp_int8")
-    x, sx = _dense(rows.codes), rows.scales.contiguous()
     y = torch.empty((m, c), dtype=torch.float16, device=dev)
     lib = _lib.lib()
     with _lib.on(dev):
@@ -222,19 +245,15 @@ def _check_width(name, width):
         raise ValueError(f"{name} of {width} channels (a multiple of 16, at most {_MOST_WIDTH})")
 
 
-def _kept_buffer(m, k, device):
-    return torch.empty(m * k + m * (k // 16), dtype=torch.uint8, device=device)
-
-
 def keep_rows(x):
     """uint8 [17 N C / 16]: fp16 rows [N,C] in eight bits, in groups of sixteen numbers: codes int8 [N,C], then a byte with the scale of
     every group (s3d_keep_rows has the form).  C is a multiple of 16, at most 16384.  x is taken as its data."""
-    _check("x", x, (torch.float16,), (None, None))
+    _check("x", x, _FP16, _ANY_ROWS)
     m, k = x.shape
     _check_width("rows", k)
     _unfollowed("keep_rows")
     x = _dense(x.detach())
-    kept = _kept_buffer(m, k, x.device)
+    kept = torch.empty(_kept_size(m, k), dtype=torch.uint8, device=x.device)
     with _lib.on(x.device):
         status = _lib.lib().s3d_keep_rows(x.data_ptr(), kept.data_ptr(), m, k, _lib.stream(x.device))
     _lib.check(status, "s3d_keep_rows")
@@ -257,15 +276,6 @@ def kept_values(kept, channels):
     return out
 
 
-def _copies(weight, bias, turned):
-    """(weight, its transpose or None, bias or None) in fp16, as the kernels read them."""
-    done = _half_copies(weight, bias, turned) if weight.dtype == torch.float32 and (bias is None or bias.dtype == torch.float32) else None
-    if done is None:
-        half = _dense(weight.to(torch.float16))
-        done = half, half.t().contiguous() if turned else None, None if bias is None else _dense(bias.to(torch.float16))
-    return done
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -284,42 +294,70 @@ def _parameter_gradients(dtypes, needs, shapes, rows, device):
     return dtype, [make(shape, dtype=dtype, device=device) if need else None for shape, need in zip(shapes, needs)]
 
 
+def _saved_places(sizes):
+    """(where blocks of as many bytes begin in one buffer, each on a multiple of 256, and its size)."""
+    places, at = [], 0
+    for size in sizes:
+        places.append(at)
+        at += size + -size % 256
+    return places, at
+
+
+def _kept_size(m, k):
+    return m * k + m * (k // 16)
+
+
+def _typed(grads, dtypes):
+    return (g if g is None or g.dtype == d else g.to(d) for g, d in zip(grads, dtypes))
+
+
 class _KeptLinear(Function):
     """graph: whether one is recorded; without it nothing is kept."""
 
     @staticmethod
     def forward(ctx, graph, x, weight, bias):
-        need_x, need_weight, _ = (graph and need for need in ctx.needs_input_grad[1:])
+        need_x, need_weight = (graph and need for need in ctx.needs_input_grad[1:3])
         (m, k), n, dev = x.shape, weight.shape[0], x.device
-        half, turned, half_bias = _copies(weight, bias, need_x)
-        rows = _dense(x)
         y = torch.empty((m, n), dtype=torch.float16, device=dev)
-        kept = _kept_buffer(m, k, dev) if need_weight else None
+        # one buffer for what the backward reads: kept rows, and the weight transposed
+        places, size = _saved_places((_kept_size(m, k) if need_weight else 0, 2 * n * k if need_x else 0))
+        saved = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         if m:
+            rows, weight, bias = _dense(x), _dense(weight), None if bias is None else _dense(bias)
+            at = saved.data_ptr() if size else 0
+            lib = _lib.lib()
+            ws_bytes = lib.s3d_kept_linear_workspace_bytes(n, k)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             with _lib.on(dev):
-                status = _lib.lib().s3d_kept_linear(rows.data_ptr(), half.data_ptr(), _ptr(half_bias), y.data_ptr(), _ptr(kept), m, n, k, _lib.stream(dev))
+                status = lib.s3d_kept_linear(
+                    rows.data_ptr(), weight.data_ptr(), _DTYPE_CODE[weight.dtype], _ptr(bias), 0 if bias is None else _DTYPE_CODE[bias.dtype],
+                    y.data_ptr(), at + places[0] if need_weight else None, at + places[1] if need_x else None, m, n, k, workspace.data_ptr(), ws_bytes,
+                    _lib.stream(dev))
             _lib.check(status, "s3d_kept_linear")
-        ctx.save_for_backward(kept, turned)
-        ctx.shapes, ctx.dtypes = (m, n, k), [None if p is None else p.dtype for p in (weight, bias)]
+        ctx.save_for_backward(saved)
+        ctx.shapes, ctx.places, ctx.dtypes = (m, n, k), places, [weight.dtype, None if bias is None else bias.dtype]
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        kept, turned = ctx.saved_tensors
-        (m, n, k), dev, needs = ctx.shapes, dy.device, ctx.needs_input_grad[1:]
-        dx = torch.empty((m, k), dtype=torch.float16, device=dev) if needs[0] else None
-        dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((n, k), (n,)), m, dev)
-        if m and (dx is not None or any(g is not None for g in grads)):
-            dy = _rows_like(dy, torch.float16)
-            lib = _lib.lib()
-            with _lib.on(dev):
-                ws_bytes = lib.s3d_kept_linear_grad_workspace_bytes(m, n, k)
-                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-                status = lib.s3d_kept_linear_grad(dy.data_ptr(), _ptr(turned), _ptr(kept), _ptr(dx), *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, n, k,
-                                                  workspace.data_ptr(), ws_bytes, _lib.stream(dev))
-            _lib.check(status, "s3d_kept_linear_grad")
-        return (None, dx, *(g if g is None or g.dtype == d else g.to(d) for g, d in zip(grads, ctx.dtypes)))
+        return _linear_gradients_once(ctx, dy) if torch.is_grad_enabled() else _linear_gradients(ctx, dy)
+
+
+def _linear_gradients(ctx, dy):
+    saved, = ctx.saved_tensors
+    (m, n, k), places, dev, needs = ctx.shapes, ctx.places, dy.device, ctx.needs_input_grad[1:]
+    dx = torch.empty((m, k), dtype=torch.float16, device=dev) if needs[0] else None
+    dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((n, k), (n,)), m, dev)
+    if m:
+        dy, at = _rows_like(dy, torch.float16), 0 if saved is None else saved.data_ptr()
+        lib = _lib.lib()
+        ws_bytes = lib.s3d_kept_linear_grad_workspace_bytes(m, n, k)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _lib.on(dev):
+            status = lib.s3d_kept_linear_grad(dy.data_ptr(), at + places[1] if needs[0] else None, at + places[0] if needs[1] else None, _ptr(dx),
+                                              *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, n, k, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+        _lib.check(status, "s3d_kept_linear_grad")
+    return (None, dx, *_typed(grads, ctx.dtypes))
 
 
 class _KeptMlp(Function):
@@ -328,42 +366,59 @@ class _KeptMlp(Function):
         needs = [graph and need for need in ctx.needs_input_grad[1:]]
         (m, c), hidden, dev = x.shape, weight1.shape[0], x.device
         behind = any(needs[:3])
-        half1, turned1, half_bias1 = _copies(weight1, bias1, needs[0])
-        half2, turned2, half_bias2 = _copies(weight2, bias2, behind)
-        rows = _dense(x)
         y = torch.empty((m, c), dtype=torch.float16, device=dev)
-        kept_x = _kept_buffer(m, c, dev) if needs[1] else None
-        kept_h = _kept_buffer(m, hidden, dev) if behind or needs[3] else None
+        wanted = needs[1], behind or needs[3], needs[0], behind
+        places, size = _saved_places([size if want else 0 for size, want in zip(
+            (_kept_size(m, c), _kept_size(m, hidden), 2 * c * hidden, 2 * c * hidden), wanted)])
+        saved = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        params = weight1, bias1, weight2, bias2
         if m:
+            rows, params = _dense(x), [None if p is None else _dense(p) for p in params]
+            at = saved.data_ptr() if size else 0
             lib = _lib.lib()
+            ws_bytes = lib.s3d_kept_mlp_workspace_bytes(m, c, hidden)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             with _lib.on(dev):
-                ws_bytes = lib.s3d_kept_mlp_workspace_bytes(m, c, hidden)
-                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-                status = lib.s3d_kept_mlp(rows.data_ptr(), half1.data_ptr(), _ptr(half_bias1), half2.data_ptr(), _ptr(half_bias2), y.data_ptr(), _ptr(kept_x),
-                                          _ptr(kept_h), m, c, hidden, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+                status = lib.s3d_kept_mlp(
+                    rows.data_ptr(), *(_ptr(p) for p in params), _dtype_codes(*(None if p is None else p.dtype for p in params)), y.data_ptr(),
+                    *(at + place if want else None for place, want in zip(places, wanted)), m, c, hidden, workspace.data_ptr(), ws_bytes,
+                    _lib.stream(dev))
             _lib.check(status, "s3d_kept_mlp")
-        ctx.save_for_backward(kept_x, kept_h, turned1, turned2)
-        ctx.shapes = (m, c, hidden)
-        ctx.dtypes = [None if p is None else p.dtype for p in (weight1, bias1, weight2, bias2)]
+        ctx.save_for_backward(saved)
+        ctx.shapes, ctx.places, ctx.wanted = (m, c, hidden), places, wanted
+        ctx.dtypes = [None if p is None else p.dtype for p in params]
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        kept_x, kept_h, turned1, turned2 = ctx.saved_tensors
-        needs, (m, c, hidden), dev = ctx.needs_input_grad[1:], ctx.shapes, dy.device
-        dx = torch.empty((m, c), dtype=torch.float16, device=dev) if needs[0] else None
-        dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((hidden, c), (hidden,), (c, hidden), (c,)), m, dev)
-        if m:
-            dy = _rows_like(dy, torch.float16)
-            lib = _lib.lib()
-            with _lib.on(dev):
-                ws_bytes = lib.s3d_kept_mlp_grad_workspace_bytes(m, c, hidden)
-                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-                status = lib.s3d_kept_mlp_grad(dy.data_ptr(), _ptr(turned1), _ptr(turned2), _ptr(kept_x), _ptr(kept_h), _ptr(dx), *(_ptr(g) for g in grads),
-                                               _DTYPE_CODE[dtype], m, c, hidden, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
-            _lib.check(status, "s3d_kept_mlp_grad")
-        return (None, dx, *(g if g is None or g.dtype == d else g.to(d) for g, d in zip(grads, ctx.dtypes)))
+        return _mlp_gradients_once(ctx, dy) if torch.is_grad_enabled() else _mlp_gradients(ctx, dy)
+
+
+def _mlp_gradients(ctx, dy):
+    saved, = ctx.saved_tensors
+    needs, (m, c, hidden), dev = ctx.needs_input_grad[1:], ctx.shapes, dy.device
+    dx = torch.empty((m, c), dtype=torch.float16, device=dev) if needs[0] else None
+    dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((hidden, c), (hidden,), (c, hidden), (c,)), m, dev)
+    if m:
+        dy, at = _rows_like(dy, torch.float16), 0 if saved is None else saved.data_ptr()
+        kept_x, kept_h, turned1, turned2 = (at + place if want else None for place, want in zip(ctx.places, ctx.wanted))
+        lib = _lib.lib()
+        ws_bytes = lib.s3d_kept_mlp_grad_workspace_bytes(m, c, hidden)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _lib.on(dev):
+            status = lib.s3d_kept_mlp_grad(dy.data_ptr(), turned1, turned2, kept_x, kept_h, _ptr(dx), *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, c,
+                                           hidden, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+        _lib.check(status, "s3d_kept_mlp_grad")
+    return (None, dx, *_typed(grads, ctx.dtypes))
+
+
+@functools.lru_cache(maxsize=32)
+def _dtype_codes(*dtypes):
+    return (ctypes.c_int32 * len(dtypes))(*(_DTYPE_CODE.get(d, 0) for d in dtypes))
+
+
+# (a graph of the gradients: they are no functions of what they are made from that autograd could follow, and say so when it tries)
+_linear_gradients_once, _mlp_gradients_once = once_differentiable(_linear_gradients), once_differentiable(_mlp_gradients)
 
 
 def _check_layer(name, weight, bias, k, dev):
@@ -383,7 +438,7 @@ def checkpointed_linear(x, weight, bias=None):
     """F.linear(x, weight, bias) in fp16 for fp16 rows [N,in] and parameters in fp16 or fp32, which keeps x for its backward in eight
     bits: 1.0625 bytes a number in place of two.  y and the gradient of x are those of the layer in fp16; the gradients of the parameters come in
     their own type, weight's from what was kept.  Widths are multiples of 16 up to 16384.  Gradients of gradients are refused."""
-    _check("x", x, (torch.float16,), (None, None))
+    _check("x", x, _FP16, _ANY_ROWS)
     _check_layer("weight", weight, bias, x.shape[1], x.device)
     _no_followers("checkpointed_linear")
     return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias)
@@ -394,7 +449,7 @@ def checkpointed_mlp(x, weight1, bias1, weight2, bias2):
     x and the hidden layer's rows in front of GELU in eight bits: for a hidden layer of 4 C channels 5.3 C bytes a row, where x and the hidden layer on both
     sides of GELU are 18 C.  The gradients go by what was kept.  Widths are multiples of 16 up to 16384, biases may be None.  Gradients of gradients
     are refused."""
-    _check("x", x, (torch.float16,), (None, None))
+    _check("x", x, _FP16, _ANY_ROWS)
     c = x.shape[1]
     _check_layer("weight1", weight1, bias1, c, x.device)
     _check_layer("weight2", weight2, bias2, weight1.shape[0], x.device)
