@@ -735,6 +735,25 @@ int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const
                  size_t workspace_bytes, void *stream);
 
 /*
+ * s3d_swin_blocks with the rows in front of every dense layer in eight bits: norms as s3d_add_norm_int8 has them, products as
+ * s3d_linear_int8 and s3d_mlp_int8, the attention in fp16 and its rows as s3d_quantize_rows has them.  C and hidden multiples of 16, at
+ * most 1024 and 8192.
+ */
+typedef struct {
+    const float *norm1_weight, *norm1_bias, *norm2_weight, *norm2_bias;   /* fp32 [C] */
+    const int8_t *qkv_weight, *proj_weight, *fc1_weight, *fc2_weight;     /* codes [3C,C], [C,C], [hidden,C], [C,hidden] */
+    const float *qkv_scales, *proj_scales, *fc1_scales, *fc2_scales;      /* a scale per output channel (those of q times D^-0.5) */
+    const float *qkv_bias, *proj_bias, *fc1_bias, *fc2_bias;              /* fp32 (that of q times D^-0.5), or null */
+    const void *table_q, *table_k, *table_v; /* fp16 [table_len] */
+    float norm1_eps, norm2_eps;
+} s3d_swin_block_int8;
+
+size_t s3d_swin_blocks_int8_workspace_bytes(int64_t N, int32_t C, int32_t hidden);
+int s3d_swin_blocks_int8(const float *x, float *x_out, void *pending, int64_t N, int32_t H, int32_t D, int32_t hidden,
+                         const int32_t *table_sizes, int32_t nd, int64_t table_len, const s3d_window_set *sets, int32_t num_sets,
+                         const s3d_swin_block_int8 *blocks, int32_t num_blocks, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Kept rows: what the backward of a layer reads of its fp16 input, in 1.0625 bytes a number.  Sixteen neighbouring numbers of a row
  * share a scale, the smallest number of four significant bits and multiple of 2^-24 with 127 scales reaching the largest of them;
  * code = x / scale to the nearest, ties to even.  What a code stands for, code times scale, is an fp16 number (at the largest scale,

@@ -12,6 +12,8 @@ from .window_index import (WindowIndex, build_window_index, build_window_indices
                            window_signals)
 from .crse import crse_table_rows, crse_table_sizes, scale_crse_coords
 from .fused_norm import add_layernorm
+from .eight_bits import (Int8Rows, add_norm_int8, checkpointed_linear, checkpointed_mlp, keep_rows, kept_values, linear_int8, mlp_int8,
+                         quantize_rows)
 
 __version__ = "0.1.0"
 
@@ -21,4 +23,5 @@ __all__ = [
     "build_window_indices", "window_signals",
     "get_index01", "sparse_self_attention", "crse_table_rows", "crse_table_sizes",
     "scale_crse_coords", "add_layernorm",
+    "Int8Rows", "add_norm_int8", "quantize_rows", "linear_int8", "mlp_int8", "keep_rows", "kept_values", "checkpointed_linear", "checkpointed_mlp",
 ]

@@ -41,6 +41,12 @@ class SwinBlock(ctypes.Structure):
                                    "fc2_weight", "fc2_bias")] + [("norm1_eps", ctypes.c_float), ("norm2_eps", ctypes.c_float)]
 
 
+class SwinBlockInt8(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("norm1_weight", "norm1_bias", "norm2_weight", "norm2_bias", "qkv_weight", "proj_weight", "fc1_weight", "fc2_weight",
+                                   "qkv_scales", "proj_scales", "fc1_scales", "fc2_scales", "qkv_bias", "proj_bias", "fc1_bias", "fc2_bias",
+                                   "table_q", "table_k", "table_v")] + [("norm1_eps", ctypes.c_float), ("norm2_eps", ctypes.c_float)]
+
+
 class HalfCopy(ctypes.Structure):
     _fields_ = [(n, _i64) for n in ("rows", "cols", "scaled_rows", "to", "transposed", "same")] + [("scale", ctypes.c_float)]
 
@@ -142,6 +148,9 @@ SIGNATURES = {
     "s3d_linear_int8": (ctypes.c_int, [_vp] * 6 + [_i64, _i32, _i32, _i32, _vp]),
     "s3d_mlp_int8_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
     "s3d_mlp_int8": (ctypes.c_int, [_vp] * 9 + [_i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_swin_blocks_int8_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
+    "s3d_swin_blocks_int8": (ctypes.c_int, [_vp] * 3 + [_i64, _i32, _i32, _i32] + [_vp, _i32, _i64] + [_vp, _i32] * 2 +
+                             [_vp, ctypes.c_size_t, _vp]),
     "s3d_kept_bytes": (ctypes.c_size_t, [_i64, _i32]),
     "s3d_keep_rows": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
     "s3d_kept_values": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),

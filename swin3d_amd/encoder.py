@@ -34,12 +34,13 @@ import torch.nn.functional as F
 
 from . import _lib
 from .crse import crse_num_axes, crse_table_sizes, scale_crse_coords
+from .eight_bits import checkpointed_linear, checkpointed_mlp
 from .fused_norm import add_half, add_layernorm, trained_add_norm
 from .linear_grad import trained_linear
 from .sparse_dl.attn.attn_coff import IndexMode, PosEmb, PrecisionMode, SelfAttnAIOFunction, TableDims
 from .sparse_dl.knn import KNN, KNNInterpolate, KNNInterpolateAdd, KNNMaxPool, interpolate_add_applies, knn_query
 from .sparse_dl.knn.knn import _max_pool
-from .swin_blocks import data_only, linear_rows, plain, swin_blocks
+from .swin_blocks import _applicable, _parts, data_only, linear_rows, plain, swin_blocks
 from .swin_train import trained_branches
 from .window_index import get_index01, index_arguments, window_signals, window_sets
 
@@ -579,12 +580,13 @@ class WindowAttention(nn.Module):
             self._cache = (key, (weight, bias, tables))
         return weight, bias, tables
 
-    def forward(self, feats, attn_args):
+    def forward(self, feats, attn_args, kept=False):
+        """kept: the projection of q, k, v keeps fp16 rows `feats` for its backward in eight bits."""
         n = feats.shape[0]
         _, _, m2w, w_sizes, w2n, n2n, w2m = attn_args[:7]
         weight, bias, tables = self._prepared()
         # q, k, v stay slices of the [N, 3C] projection output, which the attention kernels read in place
-        qkv = trained_linear(feats, weight, bias)
+        qkv = checkpointed_linear(feats, weight, bias) if kept else trained_linear(feats, weight, bias)
         qkv = F.linear(feats, weight, bias) if qkv is None else qkv
         # (unbind: its gradient is one stack, that of three slices three zeroed buffers and their sum)
         query, key, value = qkv.view(n, 3, self.num_heads, self.head_dim).unbind(1)
@@ -599,6 +601,10 @@ class WindowAttention(nn.Module):
 
 
 class SwinBlock(nn.Module):
+    # see eight_bit_inference and eight_bit_checkpoints
+    eight_bit_rows = False
+    eight_bit_kept = False
+
     def __init__(self, dim, num_heads, window_size, quant_size, mlp_ratio=4.0, cRSE="XYZ_RGB", fp16_mode=0):
         super().__init__()
         self.norm1 = nn.LayerNorm(dim)
@@ -621,6 +627,11 @@ class SwinBlock(nn.Module):
         pending is the previous block's MLP output (or None).  The residual adds and LayerNorms run as fused
         kernels that write the normalised rows in fp16, the dtype the following GEMM reads; the block's own MLP
         output is handed on as the new pending term instead of being added here."""
+        if self.eight_bit_rows:
+            whole = feats if pending is None else _plus(feats, pending)
+            done = swin_blocks(self, [self], (SwinBlock, WindowAttention, Mlp), whole, [attn_args], _cache_epoch(), None, eight_bits=True)
+            if done is not None:
+                return done
         feats, normed = add_layernorm(feats, pending, self.norm1)
         feats, normed = add_layernorm(feats, self.attn(normed, attn_args), self.norm2, inplace=pending is not None)
         return feats, self.mlp(normed)
@@ -632,6 +643,10 @@ class SwinBlock(nn.Module):
         done = trained_add_norm(feats, pending, self.norm1)
         if done is None:
             return None
+        if self.eight_bit_kept:
+            parts = _parts(self, (SwinBlock, WindowAttention, Mlp))
+            if parts is not None and _applicable([parts], feats.shape[1]):
+                return self._trained_in_eight_bits(*done, attn_args)
         whole = trained_branches(self, (SwinBlock, WindowAttention, Mlp), *done, attn_args)
         if whole is not None:
             _cache_epoch()      # (a forward that a change of parameters may follow)
@@ -643,8 +658,52 @@ class SwinBlock(nn.Module):
             return feats, self.mlp(self.norm2(feats))
         return done[0], self.mlp(done[1])
 
+    def _trained_in_eight_bits(self, feats, normed, attn_args):
+        """forward_trained behind the first norm, with what the projection of q, k, v and the MLP read of their inputs kept in eight bits.
+        (proj's input is the attention's result, which its own backward keeps.)"""
+        _cache_epoch()      # (a forward that a change of parameters may follow)
+        branch = self.attn(normed, attn_args, kept=True)
+        done = trained_add_norm(feats, branch, self.norm2)
+        feats, normed = (_plus(feats, branch), None) if done is None else done
+        normed = self.norm2(feats).to(torch.float16) if normed is None else normed
+        fc1, fc2 = self.mlp.fc1, self.mlp.fc2
+        return feats, checkpointed_mlp(normed, fc1.weight, fc1.bias, fc2.weight, fc2.bias)
+
     def _fused_path(self, feats):
         return _fused_norm_applies(feats)
+
+
+def _blocks_of(model):
+    """The Swin blocks of a network, whose widths eight bits come in."""
+    blocks = [m for m in model.modules() if isinstance(m, SwinBlock)]
+    for block in blocks:
+        widths = block.attn.dim, block.mlp.fc1.out_features
+        if any(w % 16 for w in widths):
+            raise ValueError(f"a block of {widths[0]} channels over {widths[1]}: rows in eight bits come in multiples of 16")
+    return blocks
+
+
+def eight_bit_inference(model, on=True):
+    """Inference of the model's Swin blocks under fp16 autocast with the rows in front of their dense layers, and the layers' weights, in eight bits
+    (eight_bits.py; s3d_swin_blocks_int8): a scale a row and an output channel, sums of whole numbers.  Norms, softmax, GELU and the residual stream
+    stay as they are, and so do training and inference without autocast.  Returns the model."""
+    blocks = _blocks_of(model)
+    for block in blocks:
+        widths = block.attn.dim, block.mlp.fc1.out_features
+        if widths[0] > 1024 or widths[1] > 8192:
+            raise ValueError(f"a block of {widths[0]} channels over {widths[1]}: at most 1024 and 8192 at inference")
+    for block in blocks:
+        block.eight_bit_rows = bool(on)
+    return model
+
+
+def eight_bit_checkpoints(model, on=True):
+    """Training of the model's Swin blocks under fp16 autocast with what the projection of q, k, v and the MLP read of their inputs in the backward
+    pass kept in eight bits (checkpointed_linear, checkpointed_mlp): some 22 bytes a voxel and channel in place of 36.  The forward pass is the layers'
+    in fp16; gradients go by what was kept.  Inference and training without autocast stay as they are.  Returns the model."""
+    for block in _blocks_of(model):
+        block.eight_bit_kept = bool(on)
+    return model
 
 
 class StageArguments(tuple):
@@ -745,8 +804,9 @@ class Stage(nn.Module):
         pending = None
         if len(self.blocks) > 0 and self.blocks[0]._fused_path(feats):
             epoch = _cache_epoch()
+            eight_bits = [getattr(block, "eight_bit_rows", False) for block in self.blocks]
             done = swin_blocks(self, self.blocks._modules.values(), (SwinBlock, WindowAttention, Mlp), feats, args, epoch,
-                               lambda layer: _autocast_copy(layer, epoch))
+                               lambda layer: _autocast_copy(layer, epoch), all(eight_bits)) if all(eight_bits) == any(eight_bits) else None
             if done is not None:
                 feats, pending = done
             else:

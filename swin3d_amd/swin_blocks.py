@@ -102,6 +102,37 @@ def _descriptions(parts, half_copy):
     return blocks, kept
 
 
+def _eight_bit_descriptions(parts):
+    """The blocks as s3d_swin_blocks_int8 takes them, and the tensors they point to."""
+    from .eight_bits import quantize_rows      # (which reads this module)
+    kept, blocks = [], (_lib.SwinBlockInt8 * len(parts))()
+
+    def at(t):
+        if t is None:
+            return None
+        kept.append(t)
+        return t.data_ptr()
+
+    for b, block in zip(blocks, parts):
+        _, norm1, attn, qkv, proj, norm2, _, fc1, _, fc2 = block
+        for name, layer in (("qkv", qkv), ("proj", proj), ("fc1", fc1), ("fc2", fc2)):
+            rows, bias = quantize_rows(layer.weight.detach()), None if layer.bias is None else layer.bias.detach().float().contiguous()
+            if layer is qkv:      # the scale of q
+                rows.scales[:attn.dim] *= attn.scale
+                if bias is not None:
+                    bias = bias.clone()
+                    bias[:attn.dim] *= attn.scale
+            setattr(b, name + "_weight", at(rows.codes))
+            setattr(b, name + "_scales", at(rows.scales))
+            setattr(b, name + "_bias", at(bias))
+        b.table_q, b.table_k, b.table_v = (at(attn._flat_table(kind).detach().half().contiguous()) for kind in ("query", "key", "value"))
+        for name, norm in (("norm1", norm1), ("norm2", norm2)):
+            setattr(b, name + "_weight", at(norm.weight.detach().float().contiguous()))
+            setattr(b, name + "_bias", at(norm.bias.detach().float().contiguous()))
+            setattr(b, name + "_eps", norm.eps)
+    return blocks, kept
+
+
 def _applicable(parts, channels):
     attn, fc1 = parts[0][2], parts[0][7]
     if attn.fp16_mode not in (1, 2) or attn.head_dim not in (8, 16, 32) or channels % 16 or fc1.out_features % 16:
@@ -143,7 +174,7 @@ def linear_rows(x, weight, bias, gelu=False, in_order=False):
     return out
 
 
-def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy):
+def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy, eight_bits=False):
     """(feats, pending) behind the blocks, as their `forward_fused` one after the other would give it, or None where the
     library call does not stand for them.
 
@@ -151,6 +182,7 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy):
                 parameter, its version, an attribute of a layer or `epoch` has changed
     kinds       (block, attention, MLP) types the blocks have to be of
     feats       fp32 [N,C]; left as it is
+    eight_bits  with the rows in front of the dense layers in eight bits (s3d_swin_blocks_int8)
     index_sets  per window set what index_arguments and window_signals give
     """
     n, channels = feats.shape
@@ -159,10 +191,11 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy):
     parts = [_parts(b, kinds) for b in blocks]
     if any(p is None for p in parts):
         return None
-    key = (epoch, _stamp(parts), [m for p in parts for m in p])
+    key = (epoch, eight_bits, _stamp(parts), [m for p in parts for m in p])
     kept = getattr(owner, "_s3d_blocks", None)
     if kept is None or kept.key != key:
-        kept = _Kept(key, *(_descriptions(parts, half_copy) if _applicable(parts, channels) else (None, None)))
+        describe = _eight_bit_descriptions if eight_bits else lambda parts: _descriptions(parts, half_copy)
+        kept = _Kept(key, *(describe(parts) if _applicable(parts, channels) else (None, None)))
         owner._s3d_blocks = kept
     if kept.described is None:
         return None
@@ -178,7 +211,9 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy):
     feats = feats.contiguous()
     out = torch.empty_like(feats)
     pending = torch.empty((n, channels), dtype=torch.float16, device=dev)
-    ws_bytes = lib.s3d_swin_blocks_workspace_bytes(n, channels, hidden)
+    workspace_bytes, call = (lib.s3d_swin_blocks_int8_workspace_bytes, lib.s3d_swin_blocks_int8) if eight_bits else \
+        (lib.s3d_swin_blocks_workspace_bytes, lib.s3d_swin_blocks)
+    ws_bytes = workspace_bytes(n, channels, hidden)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     sets = (_lib.WindowSet * len(index_sets))()
     held = []
@@ -201,7 +236,7 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy):
             s.w_sizes, s.w2n, s.n_coords = w_sizes.data_ptr(), w2n.data_ptr(), coords.data_ptr()
             s.n2n = None if n2n is None else n2n.data_ptr()
             s.num_windows, s.plan, s.plan_bytes = w_sizes.numel(), plan.data_ptr(), plan.numel()
-        status = lib.s3d_swin_blocks(
+        status = call(
             feats.data_ptr(), out.data_ptr(), pending.data_ptr(), n, heads, dim, hidden, c_sizes, nd, table_len, sets,
             len(sets), described, len(described), workspace.data_ptr(), ws_bytes, stream)
     _lib.check(status, "s3d_swin_blocks")
