@@ -736,8 +736,8 @@ int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const
 
 /*
  * s3d_swin_blocks with the rows in front of every dense layer in eight bits: norms as s3d_add_norm_int8 has them, products as
- * s3d_linear_int8 and s3d_mlp_int8, the attention in fp16 and its rows as s3d_quantize_rows has them.  C and hidden multiples of 16, at
- * most 1024 and 8192.
+ * s3d_linear_int8 and s3d_mlp_int8, the attention in fp16 and its rows as s3d_quantize_rows has them.  An MLP of many rows whose layers
+ * run as one kernel in fp16 (s3d_mlp, which is faster then) is that.  C and hidden multiples of 16, at most 1024 and 8192.
  */
 typedef struct {
     const float *norm1_weight, *norm1_bias, *norm2_weight, *norm2_bias;   /* fp32 [C] */
@@ -745,6 +745,7 @@ typedef struct {
     const float *qkv_scales, *proj_scales, *fc1_scales, *fc2_scales;      /* a scale per output channel (those of q times D^-0.5) */
     const float *qkv_bias, *proj_bias, *fc1_bias, *fc2_bias;              /* fp32 (that of q times D^-0.5), or null */
     const void *table_q, *table_k, *table_v; /* fp16 [table_len] */
+    const void *fc1_half, *fc1_half_bias, *fc2_half, *fc2_half_bias;      /* the MLP's layers in fp16, as for s3d_mlp */
     float norm1_eps, norm2_eps;
 } s3d_swin_block_int8;
 

@@ -44,7 +44,8 @@ class SwinBlock(ctypes.Structure):
 class SwinBlockInt8(ctypes.Structure):
     _fields_ = [(n, _vp) for n in ("norm1_weight", "norm1_bias", "norm2_weight", "norm2_bias", "qkv_weight", "proj_weight", "fc1_weight", "fc2_weight",
                                    "qkv_scales", "proj_scales", "fc1_scales", "fc2_scales", "qkv_bias", "proj_bias", "fc1_bias", "fc2_bias",
-                                   "table_q", "table_k", "table_v")] + [("norm1_eps", ctypes.c_float), ("norm2_eps", ctypes.c_float)]
+                                   "table_q", "table_k", "table_v", "fc1_half", "fc1_half_bias", "fc2_half", "fc2_half_bias")] + [
+                                       ("norm1_eps", ctypes.c_float), ("norm2_eps", ctypes.c_float)]
 
 
 class HalfCopy(ctypes.Structure):

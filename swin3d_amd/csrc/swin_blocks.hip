@@ -15,7 +15,8 @@ bool fits(int64_t N, int32_t H, int32_t D, int32_t hidden, int32_t num_sets, int
            num_sets >= 1 && num_blocks >= 1;
 }
 
-// in eight bits: rows behind a norm, or of the attention, with their scales, and q, k, v and the attention's result, or the MLP's scratch
+// in eight bits: rows behind a norm (in fp16 in front of an MLP in one kernel), or of the attention, with their scales, and q, k, v and the
+// attention's result, or the MLP's scratch
 struct EightBitPlaces {
     size_t scales, wide, total;
 };
@@ -23,8 +24,9 @@ struct EightBitPlaces {
 EightBitPlaces places_of(int64_t N, int32_t C, int32_t hidden)
 {
     EightBitPlaces p{};
-    const size_t attention = static_cast<size_t>(N) * 4 * C * 2, mlp = s3d_mlp_int8_workspace_bytes(N, C, hidden);
-    p.scales = align_up(static_cast<size_t>(N) * C, 256);
+    const bool whole = mlp_pays(N, C, hidden);
+    const size_t attention = static_cast<size_t>(N) * 4 * C * 2, mlp = whole ? 0 : s3d_mlp_int8_workspace_bytes(N, C, hidden);
+    p.scales = align_up(static_cast<size_t>(N) * C * (whole ? 2 : 1), 256);
     p.wide = p.scales + align_up(static_cast<size_t>(N) * 4, 256);
     p.total = p.wide + align_up(attention > mlp ? attention : mlp, 256);
     return p;
@@ -92,6 +94,8 @@ extern "C" __attribute__((visibility("default"))) int s3d_swin_blocks(
 
 // The same with the rows in front of every dense layer in eight bits: per block
 //   norm, qkv, attention (in fp16, as q, k, v are), its rows in eight bits, proj, add + norm, and the MLP
+// An MLP whose layers run as one kernel in fp16 (mlp.hip) stays that, since it writes no hidden layer: fp16 / eight bits, hidden = 4 C, 13.7 / 24.7 us
+// at 20,000 rows of 80, 50.7 / 57.3 at 37,499 of 192, 98 / 177 at 149,993 of 160, 130 / 310 at 595,677 of 80, 181 / 287 at 200,000 of 192.
 extern "C" __attribute__((visibility("default"))) size_t s3d_swin_blocks_int8_workspace_bytes(int64_t N, int32_t C, int32_t hidden)
 {
     using namespace s3d;
@@ -135,6 +139,12 @@ extern "C" __attribute__((visibility("default"))) int s3d_swin_blocks_int8(
             return rc;
         if (int rc = launch_quantize_rows(attended, S3D_DTYPE_F16, codes, scales, N, C, s)) return rc;
         if (int rc = launch_linear_int8({codes, b.proj_weight, scales, b.proj_scales, b.proj_bias, pending, N, C, C, false}, s)) return rc;
+        if (mlp_pays(N, C, hidden)) {
+            if (int rc = s3d_add_layernorm(from, pending, S3D_DTYPE_F16, b.norm2_weight, b.norm2_bias, b.norm2_eps, x_out, base, S3D_DTYPE_F16, N, C, stream))
+                return rc;
+            if (int rc = launch_mlp({base, b.fc1_half, b.fc1_half_bias, b.fc2_half, b.fc2_half_bias, pending, N, C, hidden}, s)) return rc;
+            continue;
+        }
         if (int rc = s3d_add_norm_int8(from, pending, S3D_DTYPE_F16, b.norm2_weight, b.norm2_bias, b.norm2_eps, 0, x_out, codes, scales, N, C, stream))
             return rc;
         if (int rc = s3d_mlp_int8(codes, scales, b.fc1_weight, b.fc1_scales, b.fc1_bias, b.fc2_weight, b.fc2_scales, b.fc2_bias, pending, N, C, hidden, wide,

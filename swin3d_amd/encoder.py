@@ -686,7 +686,8 @@ def _blocks_of(model):
 def eight_bit_inference(model, on=True):
     """Inference of the model's Swin blocks under fp16 autocast with the rows in front of their dense layers, and the layers' weights, in eight bits
     (eight_bits.py; s3d_swin_blocks_int8): a scale a row and an output channel, sums of whole numbers.  Norms, softmax, GELU and the residual stream
-    stay as they are, and so do training and inference without autocast.  Returns the model."""
+    stay as they are, and so do the MLPs of levels with so many voxels that both layers run as one kernel in fp16, training, and inference without
+    autocast.  Returns the model."""
     blocks = _blocks_of(model)
     for block in blocks:
         widths = block.attn.dim, block.mlp.fc1.out_features

@@ -125,6 +125,9 @@ def _eight_bit_descriptions(parts):
             setattr(b, name + "_weight", at(rows.codes))
             setattr(b, name + "_scales", at(rows.scales))
             setattr(b, name + "_bias", at(bias))
+            if layer in (fc1, fc2):
+                setattr(b, name + "_half", at(layer.weight.detach().half().contiguous()))
+                setattr(b, name + "_half_bias", at(None if layer.bias is None else layer.bias.detach().half()))
         b.table_q, b.table_k, b.table_v = (at(attn._flat_table(kind).detach().half().contiguous()) for kind in ("query", "key", "value"))
         for name, norm in (("norm1", norm1), ("norm2", norm2)):
             setattr(b, name + "_weight", at(norm.weight.detach().float().contiguous()))

@@ -3,7 +3,7 @@ and the gradients that come of it."""
 import pytest
 import torch
 
-from swin3d_amd import encoder, synth
+from swin3d_amd import _lib, add_layernorm, encoder, synth
 from swin3d_amd.eight_bits import add_norm_int8, linear_int8, mlp_int8, quantize_rows
 from swin3d_amd.encoder import eight_bit_checkpoints, eight_bit_inference
 from swin3d_amd.sparse_dl.attn.attn_coff import IndexMode, PosEmb, PrecisionMode, SelfAttnAIOFunction, TableDims
@@ -44,8 +44,14 @@ def _one_by_one(stage, feats, args):
             out = SelfAttnAIOFunction.apply(*qkv.unbind(1), *tables, attn.table_sizes, [None, a[3], None, a[4], a[5], a[8]], PosEmb.SEPARATE,
                                             TableDims.D0, IndexMode.INDIRECT, PrecisionMode.HALF_ALL)
         branch = linear_int8(quantize_rows(out.reshape(-1, attn.dim)), quantize_rows(block.attn.proj.weight), block.attn.proj.bias)
+        mlp, (m, c), hidden = block.mlp, feats.shape, block.mlp.fc1.out_features
+        if m >= 16384 and m >= 192 * c and c in (48, 64, 80, 96, 128, 160, 192) and hidden <= 1024:      # both layers as one kernel in fp16
+            feats, normed = add_layernorm(feats, branch, block.norm2)
+            params = [p.half() for p in (mlp.fc1.weight, mlp.fc1.bias, mlp.fc2.weight, mlp.fc2.bias)]
+            pending = torch.empty(m, c, device="cuda", dtype=torch.float16)
+            _lib.check(_lib.lib().s3d_mlp(normed.data_ptr(), *(p.data_ptr() for p in params), pending.data_ptr(), m, c, hidden, _lib.stream(feats.device)), "s3d_mlp")
+            continue
         feats, rows = add_norm_int8(feats, branch, block.norm2)
-        mlp = block.mlp
         pending = mlp_int8(rows, quantize_rows(mlp.fc1.weight), mlp.fc1.bias, quantize_rows(mlp.fc2.weight), mlp.fc2.bias)
     return feats + pending.float()
 
@@ -53,6 +59,7 @@ def _one_by_one(stage, feats, args):
 @pytest.mark.parametrize("heads,dim,window,voxels", [(6, 8, 5, 5000), (5, 16, 7, 3000), (1, 16, 5, 7), (6, 8, 5, 40000)])
 def test_blocks_at_inference(hip_lib, heads, dim, window, voxels):
     stage, coords, signals, feats = _stage(heads, dim, window, 2, voxels)
+    assert voxels != 40000 or coords.shape[0] >= 16384      # (its MLPs run as one kernel)
     stage.eval()
     with torch.no_grad():
         plan = stage.plan(coords, 1, signals)

@@ -8,7 +8,7 @@ from swin3d_amd.eight_bits import Int8Rows, add_norm_int8, linear_int8, mlp_int8
 
 pytestmark = pytest.mark.gpu
 
-WIDTHS = [4, 12, 48, 60, 64, 68, 128, 132, 256, 260, 384, 512, 516, 640, 1024, 1028, 2048, 2052, 4096, 4100, 8192]
+WIDTHS = [4, 12, 48, 60, 64, 68, 128, 132, 256, 260, 384, 512, 516, 520, 640, 768, 776, 1024, 1028, 1032, 1536, 1544, 2048, 2052, 2056, 2560, 2568, 4096, 4100, 8192]
 
 
 def _norm(kind, c, gen, eps=1e-5):
