@@ -727,7 +727,8 @@ int s3d_linear_int8(const int8_t *x, const float *x_scales, const int8_t *w, con
                     int32_t N, int32_t K, int32_t gelu, void *stream);
 /*
  * Both layers of an MLP: u = fp16(GELU(x w1^T + b1)), in eight bits as s3d_quantize_rows has them, then y = u w2^T + b2, fp16
- * [M,C].  C and hidden multiples of 16, at most 8192.
+ * [M,C], with the bits of those calls one after the other.  C and hidden multiples of 16, at most 8192.  No workspace (0 bytes, null) where
+ * both layers run as one kernel.
  */
 size_t s3d_mlp_int8_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
 int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const float *w1_scales, const float *b1, const int8_t *w2,

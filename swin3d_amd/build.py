@@ -14,7 +14,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 
 SOURCES = ["api_common.hip", "attn_fwd.hip", "attn_sweep.hip", "attn_tile.hip", "attn_strip_fwd.hip", "attn_tile_bwd.hip", "attn_strip_records.hip", "attn_strip_bwd.hip", "attn_bwd.hip",
            "window_index.hip", "knn.hip", "geometry.hip", "knn_pool_grad.hip", "layernorm.hip", "cast.hip", "linear.hip", "mlp.hip", "stem.hip", "linear_grad.hip", "swin_blocks.hip",
-           "swin_blocks_grad.hip", "norm_int8.hip", "linear_int8.hip", "kept_rows.hip", "kept_mlp.hip", "kept_grad.hip"]
+           "swin_blocks_grad.hip", "norm_int8.hip", "linear_int8.hip", "mlp_int8.hip", "kept_rows.hip", "kept_mlp.hip", "kept_grad.hip"]
 
 # packed-fp32 VALU forms are disabled for every device compilation unit
 HIPCC_FLAGS = [

@@ -34,6 +34,17 @@ bool mlp_takes(int64_t M, int32_t C, int32_t hidden);
 bool mlp_pays(int64_t M, int32_t C, int32_t hidden);      // ... and is faster than the layers apart
 int launch_mlp(const MlpArgs &a, hipStream_t stream);
 
+// Both layers of an MLP of such rows as one kernel (mlp_int8.hip), where that is faster than the layers apart
+struct MlpInt8 {
+    const int8_t *x, *w1, *w2;                  // [M,C], [hidden,C], [C,hidden]
+    const float *sx, *s1, *b1, *s2, *b2;        // [M], [hidden], [hidden] or null, [C], [C] or null
+    void *y;                                    // [M,C] fp16
+    int64_t M;
+    int32_t C, hidden;
+};
+bool mlp_int8_pays(int64_t M, int32_t C, int32_t hidden);
+int launch_mlp_int8(const MlpInt8 &a, hipStream_t stream);
+
 // Dense layers of rows in eight bits (linear_int8.hip)
 struct LinearInt8 {
     const int8_t *x, *w;              // [M,K], [N,K]

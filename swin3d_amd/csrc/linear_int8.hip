@@ -497,7 +497,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_linear_int8(const int8
 
 extern "C" __attribute__((visibility("default"))) size_t s3d_mlp_int8_workspace_bytes(int64_t M, int32_t C, int32_t hidden)
 {
-    return s3d::mlp_fits(M, C, hidden) ? s3d::places_of(M, hidden).total : 0;
+    return s3d::mlp_fits(M, C, hidden) && !s3d::mlp_int8_pays(M, C, hidden) ? s3d::places_of(M, hidden).total : 0;
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_mlp_int8(
@@ -508,6 +508,10 @@ extern "C" __attribute__((visibility("default"))) int s3d_mlp_int8(
     if (!mlp_fits(M, C, hidden))
         return fail(S3D_ERR_BAD_SHAPE, "s3d_mlp_int8: M=%lld C=%d hidden=%d (multiples of 16, at most 8192)", (long long)M, C, hidden);
     if (M == 0) return S3D_OK;
+    if (mlp_int8_pays(M, C, hidden)) {
+        if (!x || !x_scales || !w1 || !w1_scales || !w2 || !w2_scales || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_mlp_int8: null device pointer");
+        return launch_mlp_int8({x, w1, w2, x_scales, w1_scales, b1, w2_scales, b2, y, M, C, hidden}, static_cast<hipStream_t>(stream));
+    }
     const MlpPlaces p = places_of(M, hidden);
     if (!workspace || workspace_bytes < p.total)
         return fail(S3D_ERR_WORKSPACE, "s3d_mlp_int8: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);

@@ -32,7 +32,10 @@ def test_c_entry_points_refuse(hip_lib):
     for m, c, hidden in ((-1, 16, 16), (4, 24, 16), (4, 16, 24), (4, 16, 8208), (4, 8208, 16)):
         _refused(lib, lib.s3d_mlp_int8(*[one] * 9, m, c, hidden, one, 1 << 30, None), "s3d_mlp_int8: M=")
         assert lib.s3d_mlp_int8_workspace_bytes(m, c, hidden) == 0
-    _refused(lib, lib.s3d_mlp_int8(*[one] * 9, 4, 16, 16, one, 16, None), "workspace 16 B")
+    _refused(lib, lib.s3d_mlp_int8(*[one] * 9, 4, 640, 2560, one, 16, None), "workspace 16 B")
+    # both layers in one kernel: no workspace, but no null pointers
+    assert lib.s3d_mlp_int8_workspace_bytes(4, 16, 16) == 0 < lib.s3d_mlp_int8_workspace_bytes(4, 640, 2560)
+    _refused(lib, lib.s3d_mlp_int8(None, *[one] * 8, 4, 16, 16, None, 0, None), "null device pointer")
     for m, k in ((-1, 16), (4, 24), (4, 0), (4, 16400)):
         _refused(lib, lib.s3d_keep_rows(one, one, m, k, None), "s3d_keep_rows: M=")
         _refused(lib, lib.s3d_kept_values(one, one, m, k, None), "s3d_kept_values: M=")

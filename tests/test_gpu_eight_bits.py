@@ -182,6 +182,37 @@ def test_mlp_is_its_parts(hip_lib, m, c, hidden):
         assert torch.equal(mlp_int8(x, w1, bias1, w2, bias2), want)
 
 
+# widths in tiles of 32 that are not whole, wavefronts without one in either layer, more of the second layer's than the first's, 32 and 64 rows,
+# four wavefronts and eight, the last workgroup of one row, layers apart
+@pytest.mark.parametrize("m", [1, 31, 8193, 16385, 16447])
+@pytest.mark.parametrize("c,hidden", [(16, 16), (48, 16), (272, 32), (448, 48), (16, 272), (80, 320), (112, 464), (208, 416), (224, 416), (160, 624), (48, 1232),
+                                      (48, 1216), (528, 32), (256, 1024)])
+def test_mlp_of_any_width(hip_lib, m, c, hidden):
+    gen = torch.Generator(device="cuda").manual_seed(m + c)
+    x, w1, w2 = (_random_rows(n, k, gen) for n, k in ((m, c), (hidden, c), (c, hidden)))
+    b1, b2 = (torch.randn(a, device="cuda", generator=gen) for a in (hidden, c))
+    want = linear_int8(quantize_rows(linear_int8(x, w1, b1, gelu=True)), w2, b2)
+    assert torch.equal(mlp_int8(x, w1, b1, w2, b2), want)
+
+
+@pytest.mark.parametrize("m", [70, 8300, 17000])
+def test_mlp_of_rows_that_are_not_finite(hip_lib, m):
+    """A row whose scale is NaN, one whose hidden layer is beyond fp16 and one of zeros, each among others that stay what they are."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x, w1, w2 = (_random_rows(n, k, gen) for n, k in ((m, 64), (128, 64), (64, 128)))
+    b2 = torch.randn(64, device="cuda", generator=gen)
+    clean = mlp_int8(x, w1, None, w2, b2)
+    x.scales[5], x.scales[m - 1] = float("nan"), 1e9
+    x.codes[40] = 0
+    y = mlp_int8(x, w1, None, w2, b2)
+    assert y[5].isnan().all() and y[m - 1].isnan().all() and torch.equal(y[40], b2.half())
+    same = torch.ones(m, dtype=torch.bool, device="cuda")
+    same[[5, 40, m - 1]] = False
+    assert clean.isfinite().all() and torch.equal(y[same], clean[same])
+    want = linear_int8(quantize_rows(linear_int8(x, w1, None, gelu=True)), w2, b2)
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y[same], want[same])
+
+
 def test_no_rows(hip_lib):
     norm = torch.nn.LayerNorm(48, device="cuda").requires_grad_(False)
     summed, rows = add_norm_int8(torch.empty(0, 48, device="cuda"), torch.empty(0, 48, device="cuda"), norm)
