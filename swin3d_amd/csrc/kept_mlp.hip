@@ -31,9 +31,12 @@ template <int C> struct Mlp {
     static constexpr int kLds = 2 * kBuffer > kOut ? 2 * kBuffer : kOut;
 };
 
-template <int C, bool kBackward>
+enum class Way { kPlain, kKeep, kBackward };      // kPlain: nothing behind the hidden layer has a gradient
+
+template <int C, Way kWay>
 __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
 {
+    constexpr bool kBackward = kWay == Way::kBackward, kKeep = kWay == Way::kKeep;
     using L = Mlp<C>;
     __shared__ __align__(16) half8 weights_s[L::kLds];
     __shared__ __align__(16) float bias_s[kBackward ? 4 : kMostHidden];
@@ -41,8 +44,10 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
     const _Float16 *b1 = static_cast<const _Float16 *>(a.b1), *b2 = static_cast<const _Float16 *>(a.b2);
     const int M = static_cast<int>(a.M), hidden = a.hidden;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
-    const int m0 = static_cast<int>(blockIdx.x) * kRows + wave * 32, m = m0 + r32;
-    const bool inside = m < M;
+    const int m0 = static_cast<int>(blockIdx.x) * kRows + wave * 32;
+    // Lanes behind the last row do what its lanes do, stores of the same bits included: no branch around a store, behind which the compiler
+    // would wait for all stores where it has to wait for loads.
+    const int m = min(m0 + r32, M - 1);
 
     // this thread's pieces of the weights: of 32 rows of the first, which lie one after the other, and of 32 columns of the second
     const _Float16 *from[L::kLoads];
@@ -71,8 +76,8 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         for (int i = 0; i < L::kLoads; ++i) weights_s[buffer * L::kBuffer + to[i]] = held[i];
     };
     // what is kept of the hidden layer: this lane's sixteen channels of a chunk, and the bytes of its two groups
-    uint8_t *const codes_h = static_cast<uint8_t *>(a.kept_h) + static_cast<int64_t>(min(m, M - 1)) * hidden + 16 * half;
-    uint8_t *const scales_h = static_cast<uint8_t *>(a.kept_h) + static_cast<int64_t>(M) * hidden + static_cast<int64_t>(min(m, M - 1)) * (hidden / kKeptGroup);
+    uint8_t *const codes_h = static_cast<uint8_t *>(a.kept_h) + static_cast<int64_t>(m) * hidden + 16 * half;
+    uint8_t *const scales_h = static_cast<uint8_t *>(a.kept_h) + static_cast<int64_t>(M) * hidden + static_cast<int64_t>(m) * (hidden / kKeptGroup);
     uint4 codes, next_codes;
     uint32_t scales, next_scales;
     auto fetch_kept = [&](uint4 &c, uint32_t &s, int chunk) {
@@ -83,7 +88,7 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
     if (kBackward) fetch_kept(codes, scales, 0);
     half8 rows[L::kSteps];
     {
-        const _Float16 *row = x + static_cast<int64_t>(min(m, M - 1)) * C + 8 * half;
+        const _Float16 *row = x + static_cast<int64_t>(m) * C + 8 * half;
 #pragma unroll
         for (int s = 0; s < L::kSteps; ++s) rows[s] = *reinterpret_cast<const half8 *>(row + 16 * s);
     }
@@ -108,8 +113,8 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         for (int s = 0; s < L::kSteps; ++s) {
             const uint32_t byte = kept_byte(both(largest_bits(rows[s]), larger));
             const uint2 c = kept_codes(rows[s], Divisor(byte));
-            if (inside) *reinterpret_cast<uint2 *>(codes_x + 16 * s) = c;
-            if (inside && half == 0) scales_x[s] = static_cast<uint8_t>(byte);
+            *reinterpret_cast<uint2 *>(codes_x + 16 * s) = c;
+            scales_x[s] = static_cast<uint8_t>(byte);
         }
     }
     __syncthreads();
@@ -162,14 +167,10 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         word[2 * group + 1] = kept_codes(q, d);
         bytes = bytes >> 8 | byte << 24;
     };
-    const bool pairs = hidden % 64 == 0;
     auto store_kept = [&](int chunk) {
         const auto lo = __builtin_amdgcn_permlane32_swap(word[0], word[2], false, false), hi = __builtin_amdgcn_permlane32_swap(word[1], word[3], false, false);
-        if (!inside || !a.kept_h) return;
         *reinterpret_cast<uint4 *>(codes_h + chunk * kHidden) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
-        if (half) return;
-        if (!pairs) *reinterpret_cast<uint16_t *>(scales_h + chunk * 2) = static_cast<uint16_t>(bytes >> 16);
-        else if (chunk & 1) *reinterpret_cast<uint32_t *>(scales_h + chunk * 2 - 2) = bytes;
+        *reinterpret_cast<uint16_t *>(scales_h + chunk * 2) = static_cast<uint16_t>(bytes >> 16);
     };
     // hidden channels 16 s + 8 half .. + 7
     auto joined = [&](const uint2 (&v)[4], int s) {
@@ -181,7 +182,6 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
     _Float16 *const u_at = kBackward ? static_cast<_Float16 *>(a.active) + static_cast<int64_t>(m) * hidden + 8 * half : nullptr;
     auto store_hidden = [&](const half8 &terms, int chunk, int s) {
         const half8 v = joined(u, s);
-        if (!inside) return;
         *reinterpret_cast<half8 *>(dh_at + chunk * kHidden + 16 * s) = terms;
         *reinterpret_cast<half8 *>(u_at + chunk * kHidden + 16 * s) = v;
     };
@@ -215,14 +215,14 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
             if (g < 2) first_layer(next, buffer, g == 0 ? 0 : kHalf, g == 0 ? kHalf : L::kSteps);
             else second_layer(terms, 0, buffer, g == 2 ? 0 : kSome, g == 2 ? kSome : L::kTiles);
             activate(sum, t - 1, g);
-            if (!kBackward && g % 2 == 1 && a.kept_h) keep_group(g / 2);
+            if (kKeep && g % 2 == 1) keep_group(g / 2);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (kBackward) store_hidden(terms, t - 1, 0);
         terms = joined(h, 1);
         second_layer(terms, 1, buffer, 0, L::kTiles);
         if (kBackward) store_hidden(terms, t - 1, 1);
-        else store_kept(t - 1);
+        if (kKeep) store_kept(t - 1);
         sum = next;
         if (kBackward) {
             codes = next_codes;
@@ -235,9 +235,9 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         activate(sum, chunks - 1, g);
-        if (!kBackward && g % 2 == 1 && a.kept_h) keep_group(g / 2);
+        if (kKeep && g % 2 == 1) keep_group(g / 2);
     }
-    if (!kBackward) store_kept(chunks - 1);
+    if (kKeep) store_kept(chunks - 1);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const half8 terms = joined(h, s);
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
 
 template <int C> int launch(const KeptMlp &a, bool backward, hipStream_t stream)
 {
-    auto kernel = backward ? kept_mlp_kernel<C, true> : kept_mlp_kernel<C, false>;
+    auto kernel = backward ? kept_mlp_kernel<C, Way::kBackward> : a.kept_h ? kept_mlp_kernel<C, Way::kKeep> : kept_mlp_kernel<C, Way::kPlain>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(a.M, kRows))), dim3(kThreads), 0, stream, a);
     S3D_HIP_CHECK(hipGetLastError());
     return S3D_OK;

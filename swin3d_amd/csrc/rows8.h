@@ -18,10 +18,8 @@ constexpr uint32_t kKeptNaN = 255;      // of a group with a number that is not 
 
 // Three bits below five of an exponent, put where fp32 has them, are the scale but for a power of two; below the smallest exponent
 // fp32's denormal numbers continue as the scales do.  2^105 = 2^(127 - 22): bits 1 << 20 stand for 2^-129 and mean 2^-24.
-__device__ __forceinline__ float kept_scale(uint32_t byte)
-{
-    return byte == kKeptNaN ? __builtin_nanf("") : __uint_as_float(byte << 20) * 0x1p105f;
-}
+__device__ __forceinline__ float kept_step(uint32_t byte) { return __uint_as_float(byte << 20) * 0x1p105f; }
+__device__ __forceinline__ float kept_scale(uint32_t byte) { return byte == kKeptNaN ? __builtin_nanf("") : kept_step(byte); }
 
 // The byte of a group's largest size, by its fp16 bits.  Truncated, a / 127 is the scale or the one below, also where the quotient's
 // rounding crosses one; 127 times a scale is exact.
@@ -29,19 +27,19 @@ __device__ __forceinline__ uint32_t kept_byte(uint32_t largest)
 {
     const float a = __builtin_bit_cast(_Float16, static_cast<uint16_t>(largest));
     const uint32_t byte = __float_as_uint(a * (1.0f / 127.0f) * 0x1p-105f) >> 20;
-    const uint32_t up = byte + (127.0f * (__uint_as_float(byte << 20) * 0x1p105f) < a ? 1 : 0);
+    const uint32_t up = byte + (127.0f * kept_step(byte) < a ? 1 : 0);
     return largest >= 0x7c00u ? kKeptNaN : up;
 }
 
-// What turns numbers into codes of a scale
+// What turns numbers into codes of a scale.  No branch for the groups that have none: zeros are divided by the smallest scale, and what the
+// quotients of a group that is not finite are, NaN included, no code of it is above 0.
 struct Divisor {
     float scale, inverse, most;
     __device__ __forceinline__ explicit Divisor(uint32_t byte)
     {
-        const bool none = byte == 0 || byte == kKeptNaN;
-        scale = none ? 0.0f : kept_scale(byte);
-        inverse = none ? 0.0f : __builtin_amdgcn_rcpf(scale);
-        most = none ? 0.0f : byte >= 249 ? 113.0f : 127.0f;      // (114 times the largest scale, 576, would round to infinity in fp16)
+        scale = kept_step(max(byte, 1u));
+        inverse = __builtin_amdgcn_rcpf(scale);
+        most = byte == kKeptNaN ? 0.0f : byte >= 249 ? 113.0f : 127.0f;      // (114 times the largest scale, 576, would round to infinity in fp16)
     }
     // x / scale to the nearest whole number, ties to even, as the low byte of the result.  The correction makes the quotient the
     // correctly rounded one, with a reciprocal that is a unit off too; without it 2,214 of the 3,981,084 pairs of an fp16 number and a scale
