@@ -244,7 +244,6 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         second_layer(terms, s, chunks & 1, 0, L::kTiles);
         if (kBackward) store_hidden(terms, chunks - 1, s);
     }
-    if (!a.y) return;
     __syncthreads();
     // the result leaves as rows, 32 channels at a time through the wavefront's own part of LDS (no barrier)
     _Float16 *out = reinterpret_cast<_Float16 *>(weights_s) + wave * (32 * L::kOutPitch), *y = static_cast<_Float16 *>(a.y);
@@ -269,30 +268,51 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
     }
 }
 
-template <int C> int launch(const KeptMlp &a, bool backward, hipStream_t stream)
+template <int C, Way kWay> int launch(const KeptMlp &a, hipStream_t stream)
 {
-    auto kernel = backward ? kept_mlp_kernel<C, Way::kBackward> : a.kept_h ? kept_mlp_kernel<C, Way::kKeep> : kept_mlp_kernel<C, Way::kPlain>;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(a.M, kRows))), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kept_mlp_kernel<C, kWay>), dim3(static_cast<unsigned>(ceil_div(a.M, kRows))), dim3(kThreads), 0, stream, a);
     S3D_HIP_CHECK(hipGetLastError());
     return S3D_OK;
 }
 
-}  // namespace
-
-bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden, bool backward)
+bool takes(int32_t C, int32_t hidden)
 {
     const bool width = C == 48 || C == 64 || C == 80 || C == 96 || C == 128 || C == 160 || C == 192;
-    return width && hidden >= kHidden && hidden % kHidden == 0 && hidden <= kMostHidden && M >= 16384 && M >= 192 * C;
+    return width && hidden >= kHidden && hidden % kHidden == 0 && hidden <= kMostHidden;
 }
 
-int launch_kept_mlp(const KeptMlp &a, bool backward, hipStream_t stream)
+}  // namespace
+
+// A workgroup has 128 rows and goes through all hidden channels: few rows leave CUs without work, the longer the more channels there are.
+// us, two products / one kernel, hidden = 4 C: 16,384 rows of 48 17.4 / 14.9, of 96 23.1 / 25.1, 25,000 of 96 29.1 / 25.9, 20,000 of 128 30.3 / 33.5, 25,000
+// of 128 37.6 / 33.3, of 160 43.7 / 39.9, 37,499 of 160 58.0 / 57.4, of 192 64.8 / 76.1, 60,000 of 192 95.0 / 79.4, 150,000 of 160 210 / 135, 200,000 of
+// 192 334 / 261.
+bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden) { return takes(C, hidden) && M >= 16384 && 3 * M >= 4 * C * C; }
+
+// Here dh and GELU(h') leave either way, for the weights' gradients, so that it is only dh that is not read again, which GELU and its derivative,
+// bound by instructions, do not make up for where there are many channels.  us, whole call, two products / one kernel: 16,384 rows of 48 35.7 / 33.7, of 80
+// 45.2 / 45.3, 25,000 of 96 54.7 / 55.3, 37,499 of 80 59.0 / 61.9, 60,000 of 48 52.0 / 46.9, of 80 74.6 / 67.0, of 96 88.5 / 77.5, of 128 113 / 115, of 160 160 / 158,
+// of 192 193 / 213, 150,000 of 160 384 / 382, 200,000 of 192 617 / 649.
+bool kept_mlp_grad_pays(int64_t M, int32_t C, int32_t hidden) { return takes(C, hidden) && C <= 96 && M >= 16384; }
+
+int launch_kept_mlp(const KeptMlp &a, hipStream_t stream)
 {
     switch (a.C) {
-#define S3D_CASE(C) case C: return launch<C>(a, backward, stream);
+#define S3D_CASE(C) case C: return a.kept_h ? launch<C, Way::kKeep>(a, stream) : launch<C, Way::kPlain>(a, stream);
         S3D_CASE(48) S3D_CASE(64) S3D_CASE(80) S3D_CASE(96) S3D_CASE(128) S3D_CASE(160) S3D_CASE(192)
 #undef S3D_CASE
     }
     return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_mlp: C=%d", a.C);
+}
+
+int launch_kept_mlp_grad(const KeptMlp &a, hipStream_t stream)
+{
+    switch (a.C) {
+#define S3D_CASE(C) case C: return launch<C, Way::kBackward>(a, stream);
+        S3D_CASE(48) S3D_CASE(64) S3D_CASE(80) S3D_CASE(96)
+#undef S3D_CASE
+    }
+    return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_mlp_grad: C=%d", a.C);
 }
 
 }  // namespace s3d

@@ -272,7 +272,7 @@ extern "C" __attribute__((visibility("default"))) size_t s3d_kept_mlp_workspace_
 {
     if (!fits(M, hidden, C)) return 0;
     // copies of the parameters, and GELU of the hidden layer where the layers are two products
-    return copies_bytes(hidden, C) + copies_bytes(C, hidden) + (kept_mlp_pays(M, C, hidden, false) ? 0 : align_up(2 * codes_bytes(M, hidden), 256));
+    return copies_bytes(hidden, C) + copies_bytes(C, hidden) + (kept_mlp_pays(M, C, hidden) ? 0 : align_up(2 * codes_bytes(M, hidden), 256));
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2,
@@ -298,7 +298,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x
     b2 = copies.add(b2, dtypes[3], 1, C, base + whole, nullptr);
     base += copies_bytes(C, hidden);
     if (int rc = launch_copies(copies, s)) return rc;
-    if (kept_mlp_pays(M, C, hidden, false)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, M, C, hidden}, false, s);
+    if (kept_mlp_pays(M, C, hidden)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, M, C, hidden}, s);
     if (kept_x)
         if (int rc = keep(x, kept_x, M, C, s)) return rc;
     LinearArgs first{x, w1, b1, base, M, hidden, C, false};
@@ -336,9 +336,9 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
     int num = 0;
     if (dw2 || db2) grads[num++] = LinearGrad{dy, dw2 ? active : dy, dw2, db2, M, C, dw2 ? hidden : 16, 0, 1.0f};
     if (behind) {
-        if (dx && kept_mlp_pays(M, C, hidden, true)) {
+        if (dx && kept_mlp_grad_pays(M, C, hidden)) {
             const KeptMlp a{dy, w2_t, nullptr, w1_t, nullptr, dx, nullptr, const_cast<void *>(kept_h), dhidden, active, M, C, hidden};
-            if (int rc = launch_kept_mlp(a, true, s)) return rc;
+            if (int rc = launch_kept_mlp_grad(a, s)) return rc;
         } else {
             LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false};
             a.kept_grad = true;

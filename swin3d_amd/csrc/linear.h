@@ -67,9 +67,10 @@ struct KeptMlp {
     int64_t M;
     int32_t C, hidden;
 };
-bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden, bool backward);
-// the backward's x is dy, w1 and w2 are w2 and w1 transposed, y is dx; no biases
-int launch_kept_mlp(const KeptMlp &a, bool backward, hipStream_t stream);
+bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden);          // that is faster than two products
+bool kept_mlp_grad_pays(int64_t M, int32_t C, int32_t hidden);     // ... for dx and what the weights' gradients read
+int launch_kept_mlp(const KeptMlp &a, hipStream_t stream);
+int launch_kept_mlp_grad(const KeptMlp &a, hipStream_t stream);    // x is dy, w1 and w2 are w2 and w1 transposed, y is dx; no biases
 
 // A layer's weight and bias gradients (linear_grad.hip): dw = dy^T x, db = the column sums of dy; the first `scaled` rows of
 // the weight (and numbers of the bias) are parameters times `scale`
