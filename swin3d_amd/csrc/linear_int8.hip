@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kRowsThreads, 4) void linear_int8_rows_kernel(Int8A
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     const int M = a.M, N = a.N, K = a.K;
     const int sub = wave / slices.sharing, first_tile = wave % slices.sharing, rows_a_step = kRowsWaves / slices.sharing * 32;
-    const int steps = (M + rows_a_step - 1) / rows_a_step;
+    const int steps = (M - 1) / rows_a_step + 1;      // (M up to 2^31 - 1)
     int at_step = static_cast<int>(blockIdx.x);
     if (at_step >= steps) return;
 

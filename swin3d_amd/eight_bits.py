@@ -176,7 +176,7 @@ def _layer_operands(name, weight, bias, k, dev):
         raise ValueError(f"{name} takes {codes.shape[1]} channels, the rows have {k}")
     if bias is not None:
         _check(f"the bias of {name}", bias, (torch.float32, torch.float16), (n,), dev)
-        bias = _dense(bias.detach().float())
+        bias = _dense(bias.float())      # (where autograd follows it, the result requires a gradient and is refused)
     return _dense(codes), _dense(scales), bias
 
 
@@ -209,7 +209,7 @@ def linear_int8(rows, weight, bias=None, gelu=False):
     x, sx, w, sw, bias, m, k, n, dev = _product_operands(rows, weight, bias)
     if k == 0 or k % 16 or k > _MOST_SUMMED or n == 0 or n % 8:
         raise ValueError(f"a layer from {k} to {n} channels (from a multiple of 16 up to {_MOST_SUMMED}, to a multiple of 8)")
-    _unfollowed("linear_int8")
+    _unfollowed("linear_int8", bias)
     y = torch.empty((m, n), dtype=torch.float16, device=dev)
     with _lib.on(dev):
         status = _lib.lib().s3d_linear_int8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -225,7 +225,7 @@ def mlp_int8(rows, weight1, bias1, weight2, bias2):
     w2, s2, bias2 = _layer_operands("weight2", weight2, bias2, hidden, dev)
     if w2.shape[0] != c or any(w == 0 or w % 16 or w > _MOST_HIDDEN for w in (c, hidden)):
         raise ValueError(f"an MLP from {c} over {hidden} to {w2.shape[0]} channels (back to as many, multiples of 16 up to {_MOST_HIDDEN})")
-    _unfollowed("mlp_int8")
+    _unfollowed("mlp_int8", bias1, bias2)
     y = torch.empty((m, c), dtype=torch.float16, device=dev)
     lib = _lib.lib()
     with _lib.on(dev):

@@ -194,12 +194,16 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy, eight
     parts = [_parts(b, kinds) for b in blocks]
     if any(p is None for p in parts):
         return None
-    key = (epoch, eight_bits, _stamp(parts), [m for p in parts for m in p])
-    kept = getattr(owner, "_s3d_blocks", None)
+    # Codes of weights are made on the stream that reads them: another stream makes its own, and what a graph captures is made in the graph, by each
+    # replay, and kept by nobody else (until the first replay there is nothing in it).
+    captured = eight_bits and torch.cuda.is_current_stream_capturing()
+    key = (epoch, eight_bits, _lib.stream(feats.device) if eight_bits else None, _stamp(parts), [m for p in parts for m in p])
+    kept = None if captured else getattr(owner, "_s3d_blocks", None)
     if kept is None or kept.key != key:
         describe = _eight_bit_descriptions if eight_bits else lambda parts: _descriptions(parts, half_copy)
         kept = _Kept(key, *(describe(parts) if _applicable(parts, channels) else (None, None)))
-        owner._s3d_blocks = kept
+        if not captured:
+            owner._s3d_blocks = kept
     if kept.described is None:
         return None
     described, tensors = kept.described, kept.tensors

@@ -90,6 +90,35 @@ def test_blocks_at_inference(hip_lib, heads, dim, window, voxels):
         assert torch.equal(_run(stage, coords, signals, feats, plan), before)
 
 
+def test_codes_of_weights_on_other_streams_and_in_graphs(hip_lib):
+    """Codes are made on the stream that reads them; a graph's are made by its replays, from the parameters of then, and read by nobody else."""
+    stage, coords, signals, feats = _stage(6, 8, 5, 2, 3000, depth=2)
+    stage.eval()
+    eight_bit_inference(stage)
+    with torch.no_grad():
+        plan = stage.plan(coords, 1, signals)
+        want = _run(stage, coords, signals, feats, plan)
+        own = stage._s3d_blocks
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            assert torch.equal(_run(stage, coords, signals, feats, plan), want) and stage._s3d_blocks is not own
+            stage._s3d_blocks = None
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                got = _run(stage, coords, signals, feats, plan)
+            assert stage._s3d_blocks is None
+        torch.cuda.synchronize()
+        assert torch.equal(_run(stage, coords, signals, feats, plan), want)      # before the first replay
+        for factor in (1.0, 1.5, 1.0):
+            stage.blocks[0].mlp.fc1.weight.mul_(factor)
+            eager = _run(stage, coords, signals, feats, plan)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, eager) and torch.equal(got, want) == (factor == 1.0 and torch.equal(eager, want))
+            stage.blocks[0].mlp.fc1.weight.div_(factor)
+
+
 def test_without_biases_and_hooks(hip_lib):
     stage, coords, signals, feats = _stage(6, 8, 5, 2, 3000, depth=2)
     stage.eval()

@@ -311,6 +311,9 @@ def test_refusals(hip_lib):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: add_norm_int8(x.requires_grad_(), None, norm), lambda: add_norm_int8(x.detach(), None, torch.nn.LayerNorm(48, device="cuda")),
-                lambda: torch.func.vmap(quantize_rows)(torch.randn(2, 4, 48, device="cuda"))):
+                lambda: torch.func.vmap(quantize_rows)(torch.randn(2, 4, 48, device="cuda")),
+                lambda: linear_int8(rows, weight, torch.zeros(16, device="cuda", requires_grad=True)),
+                lambda: linear_int8(rows, weight, torch.zeros(16, device="cuda", dtype=torch.float16, requires_grad=True)),
+                lambda: mlp_int8(rows, weight, None, quantize_rows(torch.randn(48, 16, device="cuda")), torch.zeros(48, device="cuda", requires_grad=True))):
         with pytest.raises((RuntimeError, ValueError)):
             bad()
