@@ -8,6 +8,7 @@
 // through both, 32 hidden channels at a time, which stay in registers between the products (the halves of each sixteen change places,
 // v_permlane32_swap); weights come through LDS, the next ones on their way meanwhile.  A lane has numbers 8 g + 4 half .. + 3 of 32 hidden
 // channels of its row; sixteen channels, a group of the kept form, are in a row's two lanes.
+#include "attn_kernels.h"
 #include "linear.h"
 #include "rows8.h"
 
@@ -290,10 +291,16 @@ bool takes(int32_t C, int32_t hidden)
 bool kept_mlp_pays(int64_t M, int32_t C, int32_t hidden) { return takes(C, hidden) && M >= 16384 && 3 * M >= 4 * C * C; }
 
 // Here dh and GELU(h') leave either way, for the weights' gradients, so that it is only dh that is not read again, which GELU and its derivative,
-// bound by instructions, do not make up for where there are many channels.  us, whole call, two products / one kernel: 16,384 rows of 48 35.7 / 33.7, of 80
-// 45.2 / 45.3, 25,000 of 96 54.7 / 55.3, 37,499 of 80 59.0 / 61.9, 60,000 of 48 52.0 / 46.9, of 80 74.6 / 67.0, of 96 88.5 / 77.5, of 128 113 / 115, of 160 160 / 158,
-// of 192 193 / 213, 150,000 of 160 384 / 382, 200,000 of 192 617 / 649.
-bool kept_mlp_grad_pays(int64_t M, int32_t C, int32_t hidden) { return takes(C, hidden) && C <= 96 && M >= 16384; }
+// bound by instructions, do not make up for where there are many channels.  us, the backward's call, two products / one kernel: 16,384 rows of 48 35.7 / 33.7,
+// of 80 45.2 / 45.3, 25,000 of 96 54.7 / 55.3, 37,499 of 80 59.0 / 61.9, 60,000 of 48 52.0 / 46.9, of 80 74.6 / 67.0, of 96 88.5 / 77.5, of 192 193 / 213,
+// 200,000 of 192 617 / 649.  Of 128 and 160 channels as long as three quarters of what the chip has room for is at work (forward and backward together: 60,000
+// of 160 228 / 216, 70,000 290 / 304, of 128 218 / 227, 149,993 of 160 543 / 535, 199,327 of 128 539 / 520, 300,000 of 160 1041 / 1024).
+bool kept_mlp_grad_pays(int64_t M, int32_t C, int32_t hidden)
+{
+    if (!takes(C, hidden) || C > 160 || M < 16384) return false;
+    const int64_t groups = ceil_div(M, kRows), room = 2 * static_cast<int64_t>(device_cus());
+    return C <= 96 || 4 * groups >= 3 * room * ceil_div(groups, room);
+}
 
 int launch_kept_mlp(const KeptMlp &a, hipStream_t stream)
 {
@@ -309,7 +316,7 @@ int launch_kept_mlp_grad(const KeptMlp &a, hipStream_t stream)
 {
     switch (a.C) {
 #define S3D_CASE(C) case C: return launch<C, Way::kBackward>(a, stream);
-        S3D_CASE(48) S3D_CASE(64) S3D_CASE(80) S3D_CASE(96)
+        S3D_CASE(48) S3D_CASE(64) S3D_CASE(80) S3D_CASE(96) S3D_CASE(128) S3D_CASE(160)
 #undef S3D_CASE
     }
     return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_mlp_grad: C=%d", a.C);

@@ -120,7 +120,9 @@ def _mlp(x, w1, b1, w2, b2):
     return gelu(x @ w1.t() + b1) @ w2.t() + b2
 
 
-MLP = [(1, 16, 16), (65, 48, 192), (811, 384, 1536), (1025, 80, 160), (12421, 96, 384), (40001, 48, 192)]
+# (from 16,384 rows on: both layers in one kernel, for each width that has one, the last rows' wavefronts part full, with one row and empty)
+MLP = [(1, 16, 16), (65, 48, 192), (811, 384, 1536), (1025, 80, 160), (12421, 96, 384), (40001, 48, 192), (16385, 64, 32), (16447, 80, 320),
+       (20000, 96, 416), (60001, 128, 256), (57345, 160, 640), (49153, 192, 96), (16400, 48, 1024), (16400, 48, 1056)]
 
 
 @pytest.mark.parametrize("m,c,hidden", MLP)
@@ -216,6 +218,28 @@ def test_gradients_that_are_wanted(hip_lib, which):
             want = torch.autograd.grad(checkpointed_linear(*every), every, dz)
             got = torch.autograd.grad(checkpointed_linear(*some), [t for t, need in zip(some, needs) if need], dz)
             assert all(torch.equal(g, w) for g, w in zip(got, (w for w, need in zip(want, needs) if need)))
+
+
+@pytest.mark.parametrize("m,c,hidden", [(16391, 64, 256), (57347, 160, 320)])
+def test_gradients_that_are_wanted_of_many_rows(hip_lib, m, c, hidden):
+    """... where both layers are one kernel, which keeps a hidden layer or not, and dx is what its backward is for."""
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    tensors = [_normal(gen, m, c).half(), _normal(gen, hidden, c) / c ** 0.5, _normal(gen, hidden), _normal(gen, c, hidden) / hidden ** 0.5, _normal(gen, c)]
+    dy = _normal(gen, m, c).half()
+    with torch.no_grad():
+        y = checkpointed_mlp(*tensors)
+    want = None
+    for needs in ((1, 1, 1, 1, 1), (1, 0, 0, 0, 0), (0, 0, 0, 0, 1), (0, 0, 0, 1, 0), (0, 1, 0, 0, 0), (1, 0, 0, 1, 0)):
+        some = [t.clone().requires_grad_(bool(need)) for t, need in zip(tensors, needs)]
+        out = checkpointed_mlp(*some)
+        assert torch.equal(out, y)
+        got = torch.autograd.grad(out, [t for t, need in zip(some, needs) if need], dy)
+        if want is None:
+            want = got
+            continue
+        for g, w in zip(got, (w for w, need in zip(want, needs) if need)):
+            # without dx the hidden layer's gradient is a product of its own, whose sums have another order: a rounding to fp16 each
+            assert torch.equal(g, w) or (not needs[0] and float((g - w).norm()) <= 2.0 ** -11 * float(w.norm()))
 
 
 def test_without_biases_and_mixed_types(hip_lib):
