@@ -773,14 +773,15 @@ int s3d_kept_values(const void *kept, void *out, int64_t M, int32_t K, void *str
  * A dense layer in training that keeps its input in that form: y = x w^T + bias (fp16 [M,K], [N,K], [N] or null, [M,N]; w and bias in fp32
  * or fp16, rounded to fp16) and, unless null, kept of x and w_t, the weight transposed in fp16 [K,N].  Its gradients: dx = dy w (by w_t),
  * dw = dy^T x' and db = the column sums of dy in grad_dtype, x' what kept stands for; those that are null are left out, with kept unless dw is
- * wanted and w_t unless dx is.  M at least 1, N and K multiples of 16 up to 16384; dense and 16-byte aligned.  The same bits on every call.
+ * wanted and w_t unless dx is.  The layer's w and bias are those given, their first `scaled` rows (a multiple of 16) times scale in fp32; dw and db
+ * are of those given.  M at least 1, N and K multiples of 16 up to 16384; dense and 16-byte aligned.  The same bits on every call.
  */
 size_t s3d_kept_linear_workspace_bytes(int32_t N, int32_t K);
 int s3d_kept_linear(const void *x, const void *w, int32_t w_dtype, const void *bias, int32_t bias_dtype, void *y, void *kept, void *w_t,
-                    int64_t M, int32_t N, int32_t K, void *workspace, size_t workspace_bytes, void *stream);
+                    int64_t M, int32_t N, int32_t K, int32_t scaled, float scale, void *workspace, size_t workspace_bytes, void *stream);
 size_t s3d_kept_linear_grad_workspace_bytes(int64_t M, int32_t N, int32_t K);
 int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void *dx, void *dw, void *db, int32_t grad_dtype, int64_t M,
-                         int32_t N, int32_t K, void *workspace, size_t workspace_bytes, void *stream);
+                         int32_t N, int32_t K, int32_t scaled, float scale, void *workspace, size_t workspace_bytes, void *stream);
 /*
  * An MLP likewise: h = x w1^T + b1 (rounded to fp16), y = GELU(h) w2^T + b2, x and h kept, w1_t [C,hidden] and w2_t [hidden,C] made (each
  * unless null); dtypes HOST [4], of w1, b1, w2, b2 (that of a bias which is null is not read, but 0 or 1).  Its gradients, h' and x' what is kept:

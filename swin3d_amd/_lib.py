@@ -156,9 +156,9 @@ SIGNATURES = {
     "s3d_keep_rows": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
     "s3d_kept_values": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
     "s3d_kept_linear_workspace_bytes": (ctypes.c_size_t, [_i32, _i32]),
-    "s3d_kept_linear": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32] + [_vp] * 3 + [_i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_kept_linear": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32] + [_vp] * 3 + [_i64, _i32, _i32, _i32, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
     "s3d_kept_linear_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
-    "s3d_kept_linear_grad": (ctypes.c_int, [_vp] * 6 + [_i32, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "s3d_kept_linear_grad": (ctypes.c_int, [_vp] * 6 + [_i32, _i64, _i32, _i32, _i32, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
     "s3d_kept_mlp_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
     "s3d_kept_mlp": (ctypes.c_int, [_vp] * 11 + [_i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
     "s3d_kept_mlp_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),

@@ -57,20 +57,23 @@ struct Copies {
     const void *from[kMostCopies];
     _Float16 *to[kMostCopies], *turned[kMostCopies];      // either may be null
     int rows[kMostCopies], cols[kMostCopies], first[kMostCopies];
+    int64_t scaled[kMostCopies];                          // that many numbers are multiplied by `scale`, in fp32
     bool half[kMostCopies];
     int num, blocks;
+    float scale;
 
     // adds `from` where anything is wanted of it; what the products read of it
-    const void *add(const void *array, int32_t dtype, int32_t r, int32_t c, void *copy, void *transposed)
+    const void *add(const void *array, int32_t dtype, int32_t r, int32_t c, void *copy, void *transposed, int64_t times_scale = 0)
     {
-        const bool as_is = dtype == S3D_DTYPE_F16;
+        const bool as_is = dtype == S3D_DTYPE_F16 && times_scale == 0;
         if (!array || (as_is && !transposed)) return array;
         from[num] = array;
         to[num] = as_is ? nullptr : static_cast<_Float16 *>(copy);
         turned[num] = static_cast<_Float16 *>(transposed);
         rows[num] = r;
         cols[num] = c;
-        half[num] = as_is;
+        scaled[num] = times_scale;
+        half[num] = dtype == S3D_DTYPE_F16;
         first[num++] = blocks;
         blocks += (r + kSquare - 1) / kSquare * ((c + kSquare - 1) / kSquare);
         return as_is ? array : copy;
@@ -86,11 +89,12 @@ __global__ __launch_bounds__(kThreads) void copies_kernel(Copies a)
     const void *from = a.from[0];
     _Float16 *to = a.to[0], *turned = a.turned[0];
     int rows = a.rows[0], cols = a.cols[0], first = a.first[0];
+    int64_t scaled = a.scaled[0];
     bool half = a.half[0];
 #pragma unroll
     for (int i = 1; i < kMostCopies; ++i) {
         if (which != i) continue;
-        from = a.from[i]; to = a.to[i]; turned = a.turned[i]; rows = a.rows[i]; cols = a.cols[i]; first = a.first[i]; half = a.half[i];
+        from = a.from[i]; to = a.to[i]; turned = a.turned[i]; rows = a.rows[i]; cols = a.cols[i]; first = a.first[i]; scaled = a.scaled[i]; half = a.half[i];
     }
     const int across = (cols + kSquare - 1) / kSquare, tile = static_cast<int>(blockIdx.x) - first, r0 = tile / across * kSquare, c0 = tile % across * kSquare;
     const int four = threadIdx.x % 16 * 4;
@@ -105,6 +109,11 @@ __global__ __launch_bounds__(kThreads) void copies_kernel(Copies a)
         } else {
             const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(from) + at);
             v = half4{static_cast<_Float16>(f.x), static_cast<_Float16>(f.y), static_cast<_Float16>(f.z), static_cast<_Float16>(f.w)};
+            if (at < scaled) v = half4{to_half(f.x * a.scale), to_half(f.y * a.scale), to_half(f.z * a.scale), to_half(f.w * a.scale)};
+        }
+        if (half && at < scaled) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = to_half(static_cast<float>(v[e]) * a.scale);
         }
         if (to) *reinterpret_cast<half4 *>(to + at) = v;
         *reinterpret_cast<half4 *>(&tile_s[r][four]) = v;
@@ -141,6 +150,7 @@ dim3 grid_of(int64_t threads)
 bool rows_fit(int64_t M, int32_t K) { return M >= 0 && M <= 0x7fffffff && K >= 16 && K % 16 == 0 && K <= 16384; }
 // (M = 0 has no gradients to speak of; the callers return zeros)
 bool fits(int64_t M, int32_t N, int32_t K) { return rows_fit(M, K) && M >= 1 && N >= 16 && N % 16 == 0 && N <= 16384; }
+bool scaled_fit(int32_t scaled, int32_t N) { return scaled >= 0 && scaled <= N && scaled % 16 == 0; }
 int bad_shape(const char *who, int64_t M, int32_t N, int32_t K)
 {
     return fail(S3D_ERR_BAD_SHAPE, "%s: M=%lld, widths %d and %d (M at least 1, widths multiples of 16, at most 16384)", who, (long long)M, K, N);
@@ -220,10 +230,11 @@ extern "C" __attribute__((visibility("default"))) size_t s3d_kept_linear_workspa
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void *x, const void *w, int32_t w_dtype, const void *bias, int32_t bias_dtype,
-                                                                      void *y, void *kept, void *w_t, int64_t M, int32_t N, int32_t K, void *workspace,
-                                                                      size_t workspace_bytes, void *stream)
+                                                                      void *y, void *kept, void *w_t, int64_t M, int32_t N, int32_t K, int32_t scaled,
+                                                                      float scale, void *workspace, size_t workspace_bytes, void *stream)
 {
     if (!fits(M, N, K)) return bad_shape("s3d_kept_linear", M, N, K);
+    if (!scaled_fit(scaled, N)) return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_linear: %d scaled rows of %d (a multiple of 16)", scaled, N);
     if (!is_dtype(w_dtype) || (bias && !is_dtype(bias_dtype)))
         return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_linear: dtypes %d, %d (0 = fp32, 1 = fp16)", w_dtype, bias_dtype);
     if (!x || !w || !y) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear: null device pointer");
@@ -233,8 +244,9 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_linear(const void
     hipStream_t s = static_cast<hipStream_t>(stream);
     char *base = static_cast<char *>(workspace);
     Copies copies{};
-    w = copies.add(w, w_dtype, N, K, base, w_t);
-    bias = copies.add(bias, bias_dtype, 1, N, base + align_up(2 * static_cast<size_t>(N) * K, 256), nullptr);
+    copies.scale = scale;
+    w = copies.add(w, w_dtype, N, K, base, w_t, static_cast<int64_t>(scaled) * K);
+    bias = copies.add(bias, bias_dtype, 1, N, base + align_up(2 * static_cast<size_t>(N) * K, 256), nullptr, scaled);
     if (int rc = launch_copies(copies, s)) return rc;
     if (kept)
         if (int rc = keep(x, kept, M, K, s)) return rc;
@@ -247,10 +259,11 @@ extern "C" __attribute__((visibility("default"))) size_t s3d_kept_linear_grad_wo
 }
 
 extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void *dx, void *dw, void *db,
-                                                                           int32_t grad_dtype, int64_t M, int32_t N, int32_t K, void *workspace,
-                                                                           size_t workspace_bytes, void *stream)
+                                                                           int32_t grad_dtype, int64_t M, int32_t N, int32_t K, int32_t scaled,
+                                                                           float scale, void *workspace, size_t workspace_bytes, void *stream)
 {
     if (!fits(M, N, K)) return bad_shape("s3d_kept_linear_grad", M, N, K);
+    if (!scaled_fit(scaled, N)) return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_linear_grad: %d scaled rows of %d (a multiple of 16)", scaled, N);
     if (grad_dtype != S3D_DTYPE_F32 && grad_dtype != S3D_DTYPE_F16)
         return fail(S3D_ERR_BAD_DTYPE, "s3d_kept_linear_grad: grad_dtype %d (0 = fp32, 1 = fp16)", grad_dtype);
     if (!dy || (dx && !w_t) || (dw && !kept)) return fail(S3D_ERR_NULL_POINTER, "s3d_kept_linear_grad: null device pointer");
@@ -261,7 +274,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_linear_grad(const
     if (dx)
         if (int rc = launch_linear({dy, w_t, nullptr, dx, M, K, N, false}, s)) return rc;
     if (!dw && !db) return S3D_OK;
-    LinearGrad g{dy, dw ? kept : dy, dw, db, M, N, dw ? K : 16, 0, 1.0f};
+    LinearGrad g{dy, dw ? kept : dy, dw, db, M, N, dw ? K : 16, scaled, scale};
     g.kept = dw;
     float *parts = static_cast<float *>(workspace);
     if (int rc = launch_kept_grad_parts(&g, 1, &parts, s)) return rc;

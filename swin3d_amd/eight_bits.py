@@ -312,10 +312,10 @@ def _typed(grads, dtypes):
 
 
 class _KeptLinear(Function):
-    """graph: whether one is recorded; without it nothing is kept."""
+    """graph: whether one is recorded; without it nothing is kept.  scaled: (rows of the parameters, what they are multiplied by)."""
 
     @staticmethod
-    def forward(ctx, graph, x, weight, bias):
+    def forward(ctx, graph, x, weight, bias, scaled):
         need_x, need_weight = (graph and need for need in ctx.needs_input_grad[1:3])
         (m, k), n, dev = x.shape, weight.shape[0], x.device
         y = torch.empty((m, n), dtype=torch.float16, device=dev)
@@ -331,11 +331,11 @@ class _KeptLinear(Function):
             with _lib.on(dev):
                 status = lib.s3d_kept_linear(
                     rows.data_ptr(), weight.data_ptr(), _DTYPE_CODE[weight.dtype], _ptr(bias), 0 if bias is None else _DTYPE_CODE[bias.dtype],
-                    y.data_ptr(), at + places[0] if need_weight else None, at + places[1] if need_x else None, m, n, k, workspace.data_ptr(), ws_bytes,
-                    _lib.stream(dev))
+                    y.data_ptr(), at + places[0] if need_weight else None, at + places[1] if need_x else None, m, n, k, *scaled,
+                    workspace.data_ptr(), ws_bytes, _lib.stream(dev))
             _lib.check(status, "s3d_kept_linear")
         ctx.save_for_backward(saved)
-        ctx.shapes, ctx.places, ctx.dtypes = (m, n, k), places, [weight.dtype, None if bias is None else bias.dtype]
+        ctx.scaled, ctx.shapes, ctx.places, ctx.dtypes = scaled, (m, n, k), places, [weight.dtype, None if bias is None else bias.dtype]
         return y
 
     @staticmethod
@@ -345,7 +345,7 @@ class _KeptLinear(Function):
 
 def _linear_gradients(ctx, dy):
     saved, = ctx.saved_tensors
-    (m, n, k), places, dev, needs = ctx.shapes, ctx.places, dy.device, ctx.needs_input_grad[1:]
+    (m, n, k), places, dev, needs = ctx.shapes, ctx.places, dy.device, ctx.needs_input_grad[1:4]
     dx = torch.empty((m, k), dtype=torch.float16, device=dev) if needs[0] else None
     dtype, grads = _parameter_gradients(ctx.dtypes, needs[1:], ((n, k), (n,)), m, dev)
     if m:
@@ -355,9 +355,10 @@ def _linear_gradients(ctx, dy):
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with _lib.on(dev):
             status = lib.s3d_kept_linear_grad(dy.data_ptr(), at + places[1] if needs[0] else None, at + places[0] if needs[1] else None, _ptr(dx),
-                                              *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, n, k, workspace.data_ptr(), ws_bytes, _lib.stream(dev))
+                                              *(_ptr(g) for g in grads), _DTYPE_CODE[dtype], m, n, k, *ctx.scaled, workspace.data_ptr(), ws_bytes,
+                                              _lib.stream(dev))
         _lib.check(status, "s3d_kept_linear_grad")
-    return (None, dx, *_typed(grads, ctx.dtypes))
+    return (None, dx, *_typed(grads, ctx.dtypes), None)
 
 
 class _KeptMlp(Function):
@@ -434,14 +435,18 @@ def _no_followers(what):
         raise RuntimeError(f"{what} does not run under a transform, a forward-mode derivative, a dispatch mode or a tracer")
 
 
-def checkpointed_linear(x, weight, bias=None):
+def checkpointed_linear(x, weight, bias=None, scaled=None):
     """F.linear(x, weight, bias) in fp16 for fp16 rows [N,in] and parameters in fp16 or fp32, which keeps x for its backward in eight
     bits: 1.0625 bytes a number in place of two.  y and the gradient of x are those of the layer in fp16; the gradients of the parameters come in
-    their own type, weight's from what was kept.  Widths are multiples of 16 up to 16384.  Gradients of gradients are refused."""
+    their own type, weight's from what was kept.  scaled: (rows, factor), for a layer whose first `rows` outputs (a multiple of 16) are `factor` times
+    those of the parameters, as q's are in an attention.  Widths are multiples of 16 up to 16384.  Gradients of gradients are refused."""
     _check("x", x, _FP16, _ANY_ROWS)
     _check_layer("weight", weight, bias, x.shape[1], x.device)
     _no_followers("checkpointed_linear")
-    return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias)
+    rows, factor = (0, 1.0) if scaled is None else scaled
+    if not 0 <= rows <= weight.shape[0] or rows % 16:
+        raise ValueError(f"{rows} scaled outputs of {weight.shape[0]} (a multiple of 16)")
+    return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias, (rows, float(factor)))
 
 
 def checkpointed_mlp(x, weight1, bias1, weight2, bias2):

@@ -584,10 +584,14 @@ class WindowAttention(nn.Module):
         """kept: the projection of q, k, v keeps fp16 rows `feats` for its backward in eight bits."""
         n = feats.shape[0]
         _, _, m2w, w_sizes, w2n, n2n, w2m = attn_args[:7]
-        weight, bias, tables = self._prepared()
         # q, k, v stay slices of the [N, 3C] projection output, which the attention kernels read in place
-        qkv = checkpointed_linear(feats, weight, bias) if kept else trained_linear(feats, weight, bias)
-        qkv = F.linear(feats, weight, bias) if qkv is None else qkv
+        if kept:
+            qkv = checkpointed_linear(feats, self.qkv.weight, self.qkv.bias, (self.dim, self.scale))
+            tables = [self._flat_table(kind) for kind in ("query", "key", "value")]
+        else:
+            weight, bias, tables = self._prepared()
+            qkv = trained_linear(feats, weight, bias)
+            qkv = F.linear(feats, weight, bias) if qkv is None else qkv
         # (unbind: its gradient is one stack, that of three slices three zeroed buffers and their sum)
         query, key, value = qkv.view(n, 3, self.num_heads, self.head_dim).unbind(1)
         # the scaled signals of the index set, when the caller prepared them once for all blocks that share it

@@ -42,18 +42,21 @@ def test_c_entry_points_refuse(hip_lib):
         assert lib.s3d_kept_bytes(m, k) == 0
     assert lib.s3d_kept_bytes(100, 48) == 100 * 51
     for m, n, k in ((0, 16, 16), (4, 24, 16), (4, 16, 24), (4, 16, 16400), (4, 16400, 16)):
-        _refused(lib, lib.s3d_kept_linear(one, one, 0, None, 0, one, one, one, m, n, k, one, 1 << 30, None), "s3d_kept_linear: M=")
-        _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, m, n, k, one, 1 << 30, None), "s3d_kept_linear_grad: M=")
+        _refused(lib, lib.s3d_kept_linear(one, one, 0, None, 0, one, one, one, m, n, k, 0, 1.0, one, 1 << 30, None), "s3d_kept_linear: M=")
+        _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, m, n, k, 0, 1.0, one, 1 << 30, None), "s3d_kept_linear_grad: M=")
         _refused(lib, lib.s3d_kept_mlp(*[one] * 5, dtypes, *[one] * 5, m, k, n, one, 1 << 30, None), "s3d_kept_mlp: M=")
         _refused(lib, lib.s3d_kept_mlp_grad(*[one] * 10, 0, m, k, n, one, 1 << 30, None), "s3d_kept_mlp_grad: M=")
-    _refused(lib, lib.s3d_kept_linear(one, None, 0, None, 0, one, one, one, 4, 16, 16, one, 1 << 30, None), "null")
-    _refused(lib, lib.s3d_kept_linear(one, one, 2, None, 0, one, one, one, 4, 16, 16, one, 1 << 30, None), "dtypes 2")
-    _refused(lib, lib.s3d_kept_linear(one, one, 0, one, 5, one, one, one, 4, 16, 16, one, 1 << 30, None), "0, 5")
-    _refused(lib, lib.s3d_kept_linear(one, one, 0, None, 0, one, one, one, 4, 16, 16, one, 8, None), "workspace 8 B")
-    _refused(lib, lib.s3d_kept_linear_grad(one, one, None, one, one, one, 0, 4, 16, 16, one, 1 << 30, None), "null")
-    _refused(lib, lib.s3d_kept_linear_grad(one, None, one, one, one, one, 0, 4, 16, 16, one, 1 << 30, None), "null")
-    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 2, 4, 16, 16, one, 1 << 30, None), "grad_dtype 2")
-    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, 4, 16, 16, one, 8, None), "workspace 8 B")
+    _refused(lib, lib.s3d_kept_linear(one, None, 0, None, 0, one, one, one, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_linear(one, one, 2, None, 0, one, one, one, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "dtypes 2")
+    _refused(lib, lib.s3d_kept_linear(one, one, 0, one, 5, one, one, one, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "0, 5")
+    _refused(lib, lib.s3d_kept_linear(one, one, 0, None, 0, one, one, one, 4, 16, 16, 0, 1.0, one, 8, None), "workspace 8 B")
+    for scaled in (-16, 8, 32):
+        _refused(lib, lib.s3d_kept_linear(one, one, 0, None, 0, one, one, one, 4, 16, 16, scaled, 1.0, one, 1 << 30, None), "scaled rows")
+        _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, 4, 16, 16, scaled, 1.0, one, 1 << 30, None), "scaled rows")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, None, one, one, one, 0, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_linear_grad(one, None, one, one, one, one, 0, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "null")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 2, 4, 16, 16, 0, 1.0, one, 1 << 30, None), "grad_dtype 2")
+    _refused(lib, lib.s3d_kept_linear_grad(one, one, one, one, one, one, 0, 4, 16, 16, 0, 1.0, one, 8, None), "workspace 8 B")
     _refused(lib, lib.s3d_kept_mlp(one, one, None, None, None, dtypes, *[one] * 5, 4, 16, 16, one, 1 << 30, None), "null")
     _refused(lib, lib.s3d_kept_mlp(*[one] * 5, None, *[one] * 5, 4, 16, 16, one, 1 << 30, None), "null")
     _refused(lib, lib.s3d_kept_mlp(*[one] * 5, (ctypes.c_int32 * 4)(0, 1, 2, 0), *[one] * 5, 4, 16, 16, one, 1 << 30, None), "dtype 2")

@@ -242,6 +242,49 @@ def test_gradients_that_are_wanted_of_many_rows(hip_lib, m, c, hidden):
             assert torch.equal(g, w) or (not needs[0] and float((g - w).norm()) <= 2.0 ** -11 * float(w.norm()))
 
 
+@pytest.mark.parametrize("m,n,k,rows", [(70, 144, 48, 48), (5000, 480, 160, 160), (333, 32, 64, 32), (50, 64, 16, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_scaled_rows(hip_lib, m, n, k, rows, dtype):
+    """The layer of parameters whose first rows were multiplied by a factor, with the gradients of those that were not."""
+    gen, factor = torch.Generator(device="cuda").manual_seed(m), 8 ** -0.5
+    x, dy = _normal(gen, m, k).half(), _normal(gen, m, n).half()
+    weight, bias = (_normal(gen, n, k) / k ** 0.5).to(dtype), _normal(gen, n).to(dtype)
+    scale = torch.ones(n, device="cuda")
+    scale[:rows] = torch.tensor(factor)
+    given = [t.clone().requires_grad_() for t in (x, weight, bias)]
+    y = checkpointed_linear(*given, (rows, factor))
+    got = torch.autograd.grad(y, given, dy)
+    plain = [t.clone().requires_grad_() for t in (x, weight.float() * scale.unsqueeze(1), bias.float() * scale)]
+    want_y = checkpointed_linear(*plain)
+    want = list(torch.autograd.grad(want_y, plain, dy))
+    want[1], want[2] = (want[1] * scale.unsqueeze(1)).to(dtype), (want[2] * scale).to(dtype)
+    assert torch.equal(y, want_y) and all(torch.equal(g, w) for g, w in zip(got, want))
+    for bad in ((8, factor), (-16, factor), (n + 16, factor)):
+        with pytest.raises(ValueError):
+            checkpointed_linear(x, weight, bias, bad)
+
+
+@pytest.mark.parametrize("m,c,hidden", [(100, 48, 192), (16400, 48, 192), (50000, 160, 640)])
+def test_mlp_of_rows_that_are_not_finite(hip_lib, m, c, hidden):
+    """A row that is not finite, or whose hidden layer is not, makes its own results and the parameters' gradients NaN, and no other row's."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    params = [_normal(gen, hidden, c) / c ** 0.5, _normal(gen, hidden), _normal(gen, c, hidden) / hidden ** 0.5, _normal(gen, c)]
+    x, dy = _normal(gen, m, c).half(), _normal(gen, m, c).half()
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[[3, 64, m - 1]] = True
+    results = []
+    for rows in (x, x.clone()):
+        if results:
+            rows[3, 5], rows[64, 0], rows[m - 1] = float("nan"), float("inf"), 60000.0
+        leaves = [rows.clone().requires_grad_(), *(p.clone().requires_grad_() for p in params)]
+        y = checkpointed_mlp(*leaves)
+        results.append((y, *torch.autograd.grad(y, leaves, dy)))
+    (y, dx, *grads), (bad_y, bad_dx, *bad_grads) = results
+    assert torch.equal(y[~bad], bad_y[~bad]) and torch.equal(dx[~bad], bad_dx[~bad]) and y.isfinite().all() and dx.isfinite().all()
+    assert bad_y[bad].isnan().all() and bad_dx[bad].isnan().all()
+    assert all(g.isnan().all() for g in bad_grads[:1]) and torch.equal(bad_grads[3], grads[3])
+
+
 def test_without_biases_and_mixed_types(hip_lib):
     gen = torch.Generator(device="cuda").manual_seed(2)
     x, dy = _normal(gen, 100, 48).half(), _normal(gen, 100, 48).half()
