@@ -7,7 +7,8 @@
 // number that is not finite has codes 0 and scale NaN, so that all that is computed from it is NaN.
 //
 // Bound by memory: 4 C (+ 2 C or 4 C) bytes in, C + 4 (+ 4 C for the sum) out per row.  A row stays in registers from its loads to its
-// codes: up to 1024 channels on G lanes of a wavefront, beyond that on a workgroup, whose sums meet in LDS.
+// codes: up to 1024 channels on G lanes of a wavefront, beyond that on a workgroup, whose sums meet in LDS.  199,327 rows of 48 with an fp16
+// residual 19.2 us, 5.5 TB/s, 149,993 of 160 with an fp32 one 55.8, 5.6; 811 of 384 3.7, a launch.
 #include "linear.h"
 #include "rows8.h"
 
@@ -241,7 +242,7 @@ int launch_half(const RowArgs &a, hipStream_t stream)
     return launch_half_rows<64, 8>(a, stream);
 }
 
-// four numbers a thread
+// four numbers a thread (bound by memory: 149,993 rows of 160 to fp16 15.4 us, 4.7 TB/s)
 template <bool HALF>
 __global__ __launch_bounds__(kThreads) void values_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales, void *out, int64_t total, int fours)
 {
