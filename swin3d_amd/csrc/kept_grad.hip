@@ -29,6 +29,7 @@ struct GradArgs {
     const _Float16 *n;        // [M,N] fp16
     const void *k;            // [M,K] fp16, or kept
     float *parts;             // [splits][N K + N], turned [splits][N K + K]
+    const float *sums;        // [ceil(M / 32)][N] or null: what the columns of dY add up to over each 32 rows (not turned)
     int64_t M, rows;          // rows of a split, a multiple of a stage's
     int N, K, tiles_k, tiles, splits;
     bool turned;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(kThreads, B == 5 ? 2 : 4) void kept_grad_kernel(Gra
     float sums[kSums] = {};
 #pragma unroll
     for (int j = 0; j < B; ++j) acc[j] = f32x16{};
-    const bool sum_n = !a.turned && k0 == 0, sum_k = a.turned && n0 == 0 && wave_n == 0;
+    const bool sum_n = !a.turned && k0 == 0 && !a.sums, sum_k = a.turned && n0 == 0 && wave_n == 0;
     auto add_up = [](float &sum, const half8 &v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += static_cast<float>(v[e]);
@@ -256,6 +257,22 @@ __global__ __launch_bounds__(kThreads, B == 5 ? 2 : 4) void kept_grad_kernel(Gra
     }
     // (the same for the whole workgroup)
     if (a.turned ? n0 != 0 : k0 != 0) return;
+    if (a.sums) {
+        constexpr int kShares = kThreads / L::kN;      // (a split's rows are whole groups of 32, but for the last one's)
+        const int column = n0 + tid % L::kN;
+        const int64_t last = (end + 31) / 32;
+        float total = 0.0f;
+#pragma unroll 8
+        for (int64_t g = begin / 32 + tid / L::kN; g < last; g += kShares) total += a.sums[g * N + min(column, N - 1)];
+        __syncthreads();
+        sum[tid] = total;
+        __syncthreads();
+        if (tid >= L::kN || column >= N) return;
+#pragma unroll
+        for (int i = 1; i < kShares; ++i) total += sum[i * L::kN + tid];
+        part[static_cast<int64_t>(N) * K + column] = total;
+        return;
+    }
     const int columns = a.turned ? L::kK : L::kN, first = a.turned ? k0 : n0, width = a.turned ? K : N;
 #pragma unroll
     for (int j = 0; j < kSums; ++j) {
@@ -343,7 +360,8 @@ int launch_kept_grad_parts(LinearGrad *grads, int num, float **parts, hipStream_
         if (g.M < 1 || g.M > 0x7fffffff || g.N < 16 || g.N % 16 || g.K < 16 || g.K % 16 || g.N > 16384 || g.K > 16384)
             return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_linear_grad: M=%lld N=%d K=%d", (long long)g.M, g.N, g.K);
         const Plan p = plan_of(g.M, g.N, g.K, g.kept);
-        const GradArgs a{static_cast<const _Float16 *>(p.turned ? g.x : g.dy), p.turned ? g.dy : g.x, *parts, g.M, p.rows, p.n, p.k, p.tiles_k, p.tiles,
+        if (g.sums && p.turned) return fail(S3D_ERR_BAD_SHAPE, "s3d_kept_linear_grad: sums of %d columns beside %d", g.N, g.K);
+        const GradArgs a{static_cast<const _Float16 *>(p.turned ? g.x : g.dy), p.turned ? g.dy : g.x, *parts, p.turned ? nullptr : g.sums, g.M, p.rows, p.n, p.k, p.tiles_k, p.tiles,
                          p.splits, p.turned};
         int rc = S3D_ERR_BAD_SHAPE;
         switch (p.wn * 8 + p.b) {

@@ -129,15 +129,19 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         for (int s = begin; s < end; ++s) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at[2 * s], rows[s], sum, 0, 0, 0);
     };
     uint2 h[4], u[4];      // four numbers each: what the second layer takes, and what else leaves
+    float summed[kBackward ? 16 : 1];
+    const bool there = m0 + r32 < M;
     uint32_t word[4];
     auto activate = [&](const f32x16 &sum, int chunk, int g) {
         half4 o, v;
         if constexpr (kBackward) {
-            const float s = kept_scale(g < 2 ? scales & 0xffu : scales >> 8);
+            const float s = kept_scale(g < 2 ? scales & 0xffu : scales >> 8);      // (rows behind the last one are copies of it, for the sums nothing)
             auto one = [&](int e, float code) {
                 const Active at = gelu_and_slope(code * s);
-                o[e] = to_half(sum[4 * g + e] * at.slope);
+                const float d = sum[4 * g + e] * at.slope;
+                o[e] = to_half(d);
                 v[e] = to_half(at.value);
+                summed[4 * g + e] = there ? d : 0.0f;
             };
             one(0, code_of<0>(word[g]));
             one(1, code_of<1>(word[g]));
@@ -192,7 +196,12 @@ __global__ __launch_bounds__(kThreads, 2) void kept_mlp_kernel(const KeptMlp a)
         *reinterpret_cast<half8 *>(at) = terms;
         *reinterpret_cast<half8 *>(at + 32 * L::kOutPitch) = joined(u, s);
     };
+    float *const sums_at = kBackward ? a.sums + static_cast<int64_t>(min(m0, M - 1) / 32) * hidden + summed_column(lane) : nullptr;
     auto store_hidden = [&](int chunk) {
+        if constexpr (kBackward) {
+            const float sum = column_sum(summed, lane);
+            if (m0 < M) sums_at[chunk * kHidden] = sum;      // (the same for the whole wavefront)
+        }
         wave_fence();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {

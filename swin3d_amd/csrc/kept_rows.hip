@@ -5,7 +5,8 @@
 //            dh = (dy W2) GELU'(h');  dW2 = dy^T GELU(h');  dx = dh W1;  dW1 = dh^T x';  db2, db1 = column sums of dy, dh
 //
 // with x', h' what is kept of x and h (rounded to fp16).  Products of fp16 operands with sums in fp32; GELU(h') and dh are rounded to
-// fp16 for the products behind them.  Of an MLP with hidden = 4 C that leaves 5.3 C bytes a row for the backward, where x, h and GELU(h)
+// fp16 for the products behind them, which costs dx and dW1 as much again as their own rounding does (2.9 10^-4 of their norm for 2.1); db1 has no
+// product behind it and is the sum of dh before it is rounded.  Of an MLP with hidden = 4 C that leaves 5.3 C bytes a row for the backward, where x, h and GELU(h)
 // in fp16 are 18 C.
 #include "linear.h"
 #include "rows8.h"
@@ -184,16 +185,17 @@ size_t linear_parts_bytes(int64_t M, int32_t N, int32_t K, bool kept)
     return all > some ? all : some;
 }
 
-// GELU(h') and dh, and the parts of the weights' gradients
+// GELU(h') and dh, dh's sums over each 32 rows, and the parts of the weights' gradients
 struct MlpPlaces {
-    size_t active, dhidden, parts, total;
+    size_t active, dhidden, sums, parts, total;
 };
 MlpPlaces mlp_places(int64_t M, int32_t C, int32_t hidden)
 {
     MlpPlaces p{};
     const size_t wide = align_up(2 * codes_bytes(M, hidden), 256);
     p.dhidden = p.active + wide;
-    p.parts = p.dhidden + wide;
+    p.sums = p.dhidden + wide;
+    p.parts = p.sums + align_up(static_cast<size_t>(ceil_div(M, 32)) * hidden * 4, 256);
     p.total = p.parts + linear_parts_bytes(M, C, hidden, false) + linear_parts_bytes(M, hidden, C, true);
     return p;
 }
@@ -311,7 +313,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp(const void *x
     b2 = copies.add(b2, dtypes[3], 1, C, base + whole, nullptr);
     base += copies_bytes(C, hidden);
     if (int rc = launch_copies(copies, s)) return rc;
-    if (kept_mlp_pays(M, C, hidden)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, M, C, hidden}, s);
+    if (kept_mlp_pays(M, C, hidden)) return launch_kept_mlp({x, w1, b1, w2, b2, y, kept_x, kept_h, nullptr, nullptr, nullptr, M, C, hidden}, s);
     if (kept_x)
         if (int rc = keep(x, kept_x, M, C, s)) return rc;
     LinearArgs first{x, w1, b1, base, M, hidden, C, false};
@@ -342,6 +344,7 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
     if (!workspace || workspace_bytes < p.total)
         return fail(S3D_ERR_WORKSPACE, "s3d_kept_mlp_grad: workspace %zu B < required %zu B", workspace ? workspace_bytes : size_t(0), p.total);
     char *base = static_cast<char *>(workspace), *active = base + p.active, *dhidden = base + p.dhidden;
+    float *sums = reinterpret_cast<float *>(base + p.sums);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (!behind && dw2)
         if (int rc = values(kept_h, nullptr, active, M, hidden, s)) return rc;
@@ -350,10 +353,10 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
     if (dw2 || db2) grads[num++] = LinearGrad{dy, dw2 ? active : dy, dw2, db2, M, C, dw2 ? hidden : 16, 0, 1.0f};
     if (behind) {
         if (dx && kept_mlp_grad_pays(M, C, hidden)) {
-            const KeptMlp a{dy, w2_t, nullptr, w1_t, nullptr, dx, nullptr, const_cast<void *>(kept_h), dhidden, active, M, C, hidden};
+            const KeptMlp a{dy, w2_t, nullptr, w1_t, nullptr, dx, nullptr, const_cast<void *>(kept_h), dhidden, active, sums, M, C, hidden};
             if (int rc = launch_kept_mlp_grad(a, s)) return rc;
         } else {
-            LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false};
+            LinearArgs a{dy, w2_t, sums, dhidden, M, hidden, C, false};
             a.kept_grad = true;
             a.kept = kept_h;
             a.gelu_out = active;
@@ -364,7 +367,8 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
     }
     if (dw1 || db1) {
         grads[num] = LinearGrad{dhidden, dw1 ? kept_x : dhidden, dw1, db1, M, hidden, dw1 ? C : 16, 0, 1.0f};
-        grads[num++].kept = dw1;
+        grads[num].kept = dw1;
+        grads[num++].sums = sums;
     }
     if (num == 0) return S3D_OK;
     float *parts = reinterpret_cast<float *>(base + p.parts);

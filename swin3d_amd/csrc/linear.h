@@ -64,6 +64,7 @@ struct KeptMlp {
     void *y;                             // [M,C]
     void *kept_x, *kept_h;               // written by the forward unless null; kept_h is read by the backward
     void *dh, *active;                   // backward, [M,hidden] fp16: the hidden layer's gradients, and GELU of what is kept
+    float *sums;                         // ... [ceil(M / 32)][hidden]: the gradients' sums over each 32 rows, before they are rounded
     int64_t M;
     int32_t C, hidden;
 };
@@ -83,6 +84,7 @@ struct LinearGrad {
     const float *parts = nullptr;   // where launch_linear_grad_parts has put them, and how many
     int32_t splits = 0;
     bool kept = false;              // x in eight bits (rows8.h), for launch_kept_grad_parts
+    const float *sums = nullptr;    // [ceil(M / 32)][N], for the same: db is the sum of these, those of dy over each 32 rows before it was rounded
 };
 
 constexpr int kMostLinearGrads = 4;

@@ -30,7 +30,8 @@ static_assert(kChunk / 8 == kPieces, "pieces of eight numbers");
 __device__ __forceinline__ float gelu_erf(float x) { return (x * 0.5f) * (1.0f + erff(x * 0.70710678f)); }
 
 // The last two are of layers that keep rows in eight bits (kept_rows.hip), in `gelu_at`'s place: kKeep leaves the rows' codes and GELU of
-// the rows, rounded, in `gelu_out`; kKeptGrad multiplies by GELU's slope at what was kept, in fp32, and leaves GELU of that in `gelu_out`.
+// the rows, rounded, in `gelu_out`; kKeptGrad multiplies by GELU's slope at what was kept, in fp32, and leaves GELU of that in `gelu_out` and,
+// where `bias` points, the results' sums over each 32 rows before they are rounded, fp32 [ceil(M / 32)][N].
 enum class Behind { kNothing, kGelu, kGeluGrad, kGeluBeside, kKeep, kKeptGrad };
 
 // WM x WN wavefronts of TM x TN products of 32 x 32
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
         // the chunk is there, and nobody reads the other buffer any more
         auto meet = [&]() {
             if (inside && kBehind == Behind::kKeep && gelu_at) loads_done<TM * 2 * TN * 3>();
-            else if (inside) loads_done<TM * 2 * TN * (kBehind == Behind::kGeluBeside || kBehind == Behind::kKeptGrad ? 2 : 1)>();
+            else if (inside) loads_done<TM * 2 * TN * (kBehind == Behind::kGeluBeside || kBehind == Behind::kKeptGrad ? 2 : 1) + (kBehind == Behind::kKeptGrad ? TM * TN : 0)>();
             else loads_done<0>();
             inside = false;
             workgroup_barrier();
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 b[j][g] = half4{0, 0, 0, 0};
-                if (bias) b[j][g] = *reinterpret_cast<const half4 *>(bias + min(n0 + wave_n + j * 32 + 8 * g + 4 * half, N - 4));
+                if (kBehind != Behind::kKeptGrad && bias) b[j][g] = *reinterpret_cast<const half4 *>(bias + min(n0 + wave_n + j * 32 + 8 * g + 4 * half, N - 4));
             }
         if constexpr (kBehind == Behind::kGeluGrad) {
 #pragma unroll
@@ -199,12 +200,25 @@ __global__ __launch_bounds__(kThreads, 2) void linear_kernel(const _Float16 *__r
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const Active v = gelu_and_slope(at_codes[e] * s);
-                            o[e] = to_half(acc[i][j][4 * g + e] * v.slope);
+                            acc[i][j][4 * g + e] *= v.slope;
+                            o[e] = to_half(acc[i][j][4 * g + e]);
                             u[e] = to_half(v.value);
                         }
                         *reinterpret_cast<half4 *>(out + r32 * L::kPitch + j * 32 + 8 * g + 4 * half) = o;
                         active[j][g] = __builtin_bit_cast(uint2, u);
                     }
+                }
+                // (rows behind the last one are copies of it)
+                float *const sums = reinterpret_cast<float *>(const_cast<_Float16 *>(bias)) + static_cast<int64_t>((m0 + wave_m) / 32 + i) * N + n0 + wave_n;
+                const bool there = m0 + wave_m + i * 32 + r32 < M;
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    float v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = inside || there ? acc[i][j][e] : 0.0f;
+                    const float sum = column_sum(v, lane);
+                    const int n = j * 32 + summed_column(lane);
+                    if (inside || (m0 + wave_m + i * 32 < M && n0 + wave_n + n < N)) sums[n] = sum;
                 }
 #pragma unroll
                 for (int which = 0; which < 2; ++which) {

@@ -109,6 +109,39 @@ __device__ __forceinline__ _Float16 to_half(float v)
     return static_cast<_Float16>(v);
 }
 
+// The sums over a product's 32 rows of what its lanes hold in fp32, row lane % 32 and columns 8 g + 4 half + e as v[4 g + e]: in every lane that of column
+// summed_column(lane).  Lanes trade half of their numbers for the partner's other half, so that 16 numbers a lane are 38 instructions, where all in
+// all lanes would be 96.
+template <int kControl> __device__ __forceinline__ float from_lane(float v)
+{
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), kControl, 0xf, 0xf, true));
+}
+template <int kControl, int N> __device__ __forceinline__ void traded(float *v, bool upper)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float own = upper ? v[i + N] : v[i], other = upper ? v[i] : v[i + N];
+        v[i] = own + from_lane<kControl>(other);
+    }
+}
+__device__ __forceinline__ float column_sum(float (&v)[16], int lane)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
+        v[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+    traded<0x128, 4>(v, lane & 8);      // lanes 8 apart, then mirrored ones of eight, then two apart
+    traded<0x141, 2>(v, lane & 4);
+    traded<0x4e, 1>(v, lane & 2);
+    return v[0] + from_lane<0xb1>(v[0]);
+}
+__device__ __forceinline__ int summed_column(int lane)
+{
+    const int i = (lane & 31) >> 1;
+    return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+}
+
 // x Phi(x) and its derivative at once, of numbers that are finite or NaN: in the terms of gelu_slope, u phi(u) M(u) is what x Phi(x)
 // is below the larger of x and 0.
 struct Active {

@@ -171,6 +171,31 @@ def test_mlp(hip_lib, m, c, hidden, dtype):
     assert all(torch.equal(p, q) for p, q in zip(again, (dx, *grads)))
 
 
+@pytest.mark.parametrize("m,c,hidden", [(1, 16, 16), (31, 48, 96), (33, 80, 176), (700, 48, 192), (811, 384, 768), (12421, 96, 384), (16385, 48, 160), (20001, 96, 384),
+                                        (57345, 160, 320), (3000, 640, 1280)])
+@pytest.mark.parametrize("dx_too", [True, False])
+def test_bias_behind_gelu_is_summed_before_rounding(hip_lib, m, c, hidden, dx_too):
+    """The hidden layer's gradients are fp16 numbers for the products behind them alone: db1 is the sum of what they are rounded from.  Numbers of which
+    each is half a step above an fp16 number all round the same way: db1 of rounded ones is 2^-12 of it off or more, that of the sums an fp32 one's error."""
+    gen = torch.Generator(device="cuda").manual_seed(m + c)
+    x = torch.zeros(m, c, device="cuda").half().requires_grad_(dx_too)
+    b1 = torch.full((hidden,), 12.0, device="cuda")                    # GELU's slope there is 1 to fp32
+    # dy w2: 1 + 2^-11 + 2^-13, which fp16 rounds to 1 + 2^-10
+    w2 = torch.zeros(c, hidden, device="cuda")
+    w2[0], w2[1], w2[2] = 1.0, 2.0 ** -11, 2.0 ** -13
+    dy = torch.zeros(m, c, device="cuda").half()
+    dy[:, :3] = 1.0
+    sign = torch.randint(0, 2, (m, 1), device="cuda", generator=gen) * 2 - 1
+    w1, b2 = torch.zeros(hidden, c, device="cuda"), torch.zeros(c, device="cuda")
+    params = [p.requires_grad_() for p in (w1, b1, w2, b2)]
+    for rows in (dy, dy * sign):
+        y = checkpointed_mlp(x, *params)
+        db1 = torch.autograd.grad(y, params[1:2] if not dx_too else [x, params[1]], rows)[-1]
+        want = (1 + 2.0 ** -11 + 2.0 ** -13) * rows[:, 0].double().sum()
+        # sums of some hundred groups of 32 equal numbers, whose roundings are a unit of the sum so far each
+        assert bool(((db1.double() - want).abs() <= 2.0 ** -23 * (8 + m / 256) * m ** 0.5 + 2.0 ** -23 * want.abs() * 8).all()), (db1[:3], want)
+
+
 def test_gradients_against_differences(hip_lib):
     """Where what is kept is what was there, the gradients are those of the layers: against differences in 64 bits."""
     gen = torch.Generator(device="cuda").manual_seed(8)
