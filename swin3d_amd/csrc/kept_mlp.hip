@@ -9,8 +9,8 @@
 // v_permlane32_swap); weights come through LDS, the next ones on their way meanwhile.  A lane has numbers 8 g + 4 half .. + 3 of 32 hidden
 // channels of its row; sixteen channels, a group of the kept form, are in a row's two lanes.
 //
-// Bound by instructions, of GELU, its derivative and the codes, and by what leaves: 149,993 rows of 160 over 640 forward 174 us (0.35 of 1.36 PFLOP/s, 1.3
-// TB/s; without codes 25 less), backward 225 (2.6 TB/s).
+// Bound by instructions, of GELU, its derivative and the codes, and by what leaves: 149,993 rows of 160 over 640 forward 165 us (0.37 of 1.36 PFLOP/s, 1.4
+// TB/s; without codes 25 less), backward 227 (2.6 TB/s; dh's sums in fp32 are 1 to 4% of the call).
 #include "attn_kernels.h"
 #include "linear.h"
 #include "rows8.h"
