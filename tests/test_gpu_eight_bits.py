@@ -317,3 +317,31 @@ def test_refusals(hip_lib):
                 lambda: mlp_int8(rows, weight, None, quantize_rows(torch.randn(48, 16, device="cuda")), torch.zeros(48, device="cuda", requires_grad=True))):
         with pytest.raises((RuntimeError, ValueError)):
             bad()
+
+
+def test_offsets_beyond_32_bits(hip_lib):
+    """Arrays of more than 2^31 numbers: the last rows' results are those of the same rows by themselves."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    c, last = 512, 20000
+    m = 2 ** 31 // c + 40001
+    x = torch.zeros(m, c, device="cuda")
+    x[-last:] = torch.randn(last, c, device="cuda", generator=gen)
+    norm = torch.nn.LayerNorm(c, device="cuda").requires_grad_(False)
+    summed, rows = add_norm_int8(x, x[:1].half().expand(m, c), norm)
+    want_sum, want = add_norm_int8(x[-last:].clone(), None, norm)
+    assert torch.equal(summed[-last:], want_sum) and all(torch.equal(a[-last:], b) for a, b in zip(rows, want))
+    del x, summed
+    weight, bias = _random_rows(64, c, gen), torch.randn(64, device="cuda", generator=gen)
+    assert torch.equal(linear_int8(rows, weight, bias)[-last:], linear_int8(want, weight, bias))
+    assert torch.equal(rows.values()[-last:], want.values())
+    del rows, want
+    # more results than 2^31, by each of the kernels for many rows
+    for k, n in ((64, 512), (512, 512)):
+        rows, weight = _random_rows(m, k, gen), _random_rows(n, k, gen)
+        y = linear_int8(rows, weight)
+        tail = Int8Rows(rows.codes[-last:].clone(), rows.scales[-last:].clone())
+        assert torch.equal(y[-last:], linear_int8(tail, weight))
+        del y
+    weight2 = _random_rows(512, 64, gen)
+    y = mlp_int8(rows, _random_rows(64, 512, torch.Generator(device="cuda").manual_seed(1)), None, weight2, None)
+    assert torch.equal(y[-last:], mlp_int8(tail, _random_rows(64, 512, torch.Generator(device="cuda").manual_seed(1)), None, weight2, None))

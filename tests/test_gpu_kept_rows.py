@@ -409,3 +409,25 @@ def test_refusals(hip_lib):
     dw, = torch.autograd.grad(checkpointed_linear(x, w, b), w, torch.ones(4, 16, device="cuda").half(), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dw.sum(), w)
+
+
+@pytest.mark.parametrize("c,hidden", [(80, 640), (208, 640)])
+def test_offsets_beyond_32_bits(hip_lib, c, hidden):
+    """A hidden layer of more than 2^31 numbers, in one kernel and in two: the last rows' results are those of the same rows by themselves, and gradients
+    of parameters that come of these rows alone theirs."""
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    m, last = 2 ** 31 // hidden + 40001, 40000
+    x, dy = torch.zeros(m, c, device="cuda", dtype=torch.float16), torch.zeros(m, c, device="cuda", dtype=torch.float16)
+    x[-last:], dy[-last:] = _normal(gen, last, c).half(), _normal(gen, last, c).half()
+    params = [(_normal(gen, hidden, c) / c ** 0.5).requires_grad_(), _normal(gen, hidden).requires_grad_(),
+              (_normal(gen, c, hidden) / hidden ** 0.5).requires_grad_(), _normal(gen, c).requires_grad_()]
+
+    def passed(x, dy):
+        x = x.requires_grad_()
+        y = checkpointed_mlp(x, *params)
+        return (y[-last:].clone(), *(g[-last:].clone() if i == 0 else g for i, g in enumerate(torch.autograd.grad(y, [x, *params], dy))))
+
+    got, want = passed(x, dy), passed(x[-last:].detach().clone(), dy[-last:].clone())
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # other shares of the rows: the sums of 40,000 products in another order, some of them with zeros in between
+    assert all(float((g - w).norm()) <= 2.0 ** -18 * float(w.norm()) for g, w in zip(got[2:], want[2:]))
