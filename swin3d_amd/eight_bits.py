@@ -109,6 +109,16 @@ def _empty_rows(n, c, device):
     return Int8Rows(torch.empty((n, c), dtype=torch.int8, device=device), torch.empty(n, dtype=torch.float32, device=device))
 
 
+def _norm_parameters(norm, rms, c, dev):
+    """(weight, bias) of a norm over c channels, either may be None.  normalized_shape is a plain attribute and says nothing of what the parameters
+    are by now: the kernel reads c numbers of each."""
+    weight, bias = norm.weight, None if rms else norm.bias
+    for name, p in (("norm.weight", weight), ("norm.bias", bias)):
+        if p is not None and not (p.dtype is torch.float32 and p.device == dev and p.shape == (c,)):
+            _check(name, p, (torch.float32, torch.float16, torch.bfloat16, torch.float64), (c,), dev)
+    return weight, bias
+
+
 def add_norm_int8(x, residual, norm, inplace=False):
     """(x + residual, norm(x + residual) in eight bits) for x fp32 [N,C] and `norm` a torch.nn.LayerNorm or RMSNorm over C.
 
@@ -124,10 +134,7 @@ def add_norm_int8(x, residual, norm, inplace=False):
     rms = isinstance(norm, nn.RMSNorm)
     if not (rms or isinstance(norm, nn.LayerNorm)) or tuple(norm.normalized_shape) != (c,):
         raise ValueError(f"norm must be a LayerNorm or RMSNorm over the {c} channels, got {norm}")
-    weight, bias = norm.weight, None if rms else norm.bias
-    for name, p in (("norm.weight", weight), ("norm.bias", bias)):
-        if p is not None and not (p.dtype is torch.float32 and p.device == dev and p.dim() == 1):      # (its size is normalized_shape's)
-            _check(name, p, (torch.float32, torch.float16, torch.bfloat16, torch.float64), (c,), dev)
+    weight, bias = _norm_parameters(norm, rms, c, dev)
     if residual is not None:
         _check("residual", residual, _EITHER, (n, c), dev)
     _unfollowed("add_norm_int8", x, residual, weight, bias)

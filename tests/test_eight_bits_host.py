@@ -90,3 +90,17 @@ def test_statement_of_the_kept_form():
     values = kept(x)
     assert torch.equal(values.half().double(), values) and int(keep(x)[0].abs().max()) == 127
     assert torch.equal(values[1, :17], x[1, :17].double())
+
+
+@pytest.mark.parametrize("name", ["weight", "bias"])
+def test_parameters_that_are_not_as_long_as_the_norm_says(name):
+    """The kernel reads a number a channel of each, whatever normalized_shape still is."""
+    norm, device = torch.nn.LayerNorm(48), torch.device("cpu")
+    assert all(a is b for a, b in zip(eight_bits._norm_parameters(norm, False, 48, device), (norm.weight, norm.bias)))
+    assert eight_bits._norm_parameters(norm, True, 48, device)[1] is None
+    for other in (torch.ones(44), torch.ones(0), torch.ones(96), torch.ones(48, 1)):
+        changed = torch.nn.LayerNorm(48)
+        getattr(changed, name).data = other
+        assert tuple(changed.normalized_shape) == (48,)
+        with pytest.raises(ValueError):
+            eight_bits._norm_parameters(changed, False, 48, device)

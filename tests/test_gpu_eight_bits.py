@@ -345,3 +345,14 @@ def test_offsets_beyond_32_bits(hip_lib):
     weight2 = _random_rows(512, 64, gen)
     y = mlp_int8(rows, _random_rows(64, 512, torch.Generator(device="cuda").manual_seed(1)), None, weight2, None)
     assert torch.equal(y[-last:], mlp_int8(tail, _random_rows(64, 512, torch.Generator(device="cuda").manual_seed(1)), None, weight2, None))
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_norms_whose_parameters_are_not_as_long_as_they_say(hip_lib, kind):
+    x = torch.randn(4, 48, device="cuda")
+    for name in ("weight", "bias")[:1 if kind == "rms" else 2]:
+        for other in (torch.ones(44, device="cuda"), torch.ones(0, device="cuda"), torch.ones(96, device="cuda"), torch.ones(47, device="cuda").half()):
+            norm = _norm(kind, 48, torch.Generator(device="cuda").manual_seed(1))
+            getattr(norm, name).data = other
+            with pytest.raises(ValueError):
+                add_norm_int8(x, None, norm)
