@@ -73,8 +73,13 @@ def _check(name, t, dtypes, shape, device=None):
         kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         where = "on a CUDA (HIP) device" if device is None else f"on {device}"
         raise ValueError(f"{name} must be {kinds} [{wanted}] {where}, got {t.dtype} {tuple(sizes)} on {t.device}")
-    if sizes[0] > 0x7fffffff:
-        raise ValueError(f"{name} has {sizes[0]} rows (at most 2^31 - 1)")
+    if len(shape) == 2:
+        _check_row_count(name, sizes[0])
+
+
+def _check_row_count(name, count):
+    if count > 0x7fffffff:
+        raise ValueError(f"{name} has {count} rows (at most 2^31 - 1)")
 
 
 def _check_rows(name, rows, device=None):
@@ -274,6 +279,7 @@ def kept_values(kept, channels):
     m, rest = divmod(kept.numel(), channels + channels // 16)
     if rest:
         raise ValueError(f"{kept.numel()} bytes are no whole number of rows of {channels} channels")
+    _check_row_count("kept", m)
     _unfollowed("kept_values")
     kept = _dense(kept)
     out = torch.empty((m, channels), dtype=torch.float16, device=kept.device)

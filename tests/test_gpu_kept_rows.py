@@ -431,3 +431,16 @@ def test_offsets_beyond_32_bits(hip_lib, c, hidden):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     # other shares of the rows: the sums of 40,000 products in another order, some of them with zeros in between
     assert all(float((g - w).norm()) <= 2.0 ** -18 * float(w.norm()) for g, w in zip(got[2:], want[2:]))
+
+
+def test_form_of_more_than_32_bits_of_bytes(hip_lib):
+    """Rows whose kept form has more than 2^31 bytes: the last ones' are those of the same rows by themselves, both ways."""
+    c, last = 640, 5000
+    m = (2 ** 31 // (c + c // GROUP)) + last
+    x = torch.zeros(m, c, device="cuda", dtype=torch.float16)
+    x[-last:] = _normal(torch.Generator(device="cuda").manual_seed(9), last, c).half()
+    got, tail = keep_rows(x), keep_rows(x[-last:].clone())
+    assert got.numel() > 2 ** 31
+    assert torch.equal(got[(m - last) * c:m * c], tail[:last * c]) and torch.equal(got[-last * (c // GROUP):], tail[last * c:])
+    values = kept_values(got, c)
+    assert values.shape == x.shape and torch.equal(values[-last:], kept_values(tail, c)) and not values[:-last].any()
