@@ -40,13 +40,14 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor
 
     def values(self, dtype=torch.float16):
-        """[N,C] in float16 or float32: what the rows stand for."""
+        """[N,C] in float16 or float32: what the rows stand for.  No autograd."""
         _check_rows("rows", self)
         if dtype not in _DTYPE_CODE:
             raise ValueError(f"dtype {dtype} (float16 or float32)")
         n, c = self.codes.shape
         if c == 0 or c % 4 or c > _MOST_CHANNELS:
             raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
+        _unfollowed("Int8Rows.values", self.scales)
         dev = self.codes.device
         codes, scales = _dense(self.codes), _dense(self.scales)
         out = torch.empty((n, c), dtype=dtype, device=dev)
@@ -221,7 +222,7 @@ def linear_int8(rows, weight, bias=None, gelu=False):
     x, sx, w, sw, bias, m, k, n, dev = _product_operands(rows, weight, bias)
     if k == 0 or k % 16 or k > _MOST_SUMMED or n == 0 or n % 8:
         raise ValueError(f"a layer from {k} to {n} channels (from a multiple of 16 up to {_MOST_SUMMED}, to a multiple of 8)")
-    _unfollowed("linear_int8", bias)
+    _unfollowed("linear_int8", sx, sw, bias)
     y = torch.empty((m, n), dtype=torch.float16, device=dev)
     with _lib.on(dev):
         status = _lib.lib().s3d_linear_int8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -237,7 +238,7 @@ def mlp_int8(rows, weight1, bias1, weight2, bias2):
     w2, s2, bias2 = _layer_operands("weight2", weight2, bias2, hidden, dev)
     if w2.shape[0] != c or any(w == 0 or w % 16 or w > _MOST_HIDDEN for w in (c, hidden)):
         raise ValueError(f"an MLP from {c} over {hidden} to {w2.shape[0]} channels (back to as many, multiples of 16 up to {_MOST_HIDDEN})")
-    _unfollowed("mlp_int8", bias1, bias2)
+    _unfollowed("mlp_int8", sx, s1, bias1, s2, bias2)
     y = torch.empty((m, c), dtype=torch.float16, device=dev)
     lib = _lib.lib()
     with _lib.on(dev):

@@ -356,3 +356,19 @@ def test_norms_whose_parameters_are_not_as_long_as_they_say(hip_lib, kind):
             getattr(norm, name).data = other
             with pytest.raises(ValueError):
                 add_norm_int8(x, None, norm)
+
+
+def test_scales_that_require_a_gradient(hip_lib):
+    """Scales are numbers that a program may train.  No call has their gradient: none drops it without a word."""
+    rows, w1, w2 = (quantize_rows(torch.randn(n, k, device="cuda")) for n, k in ((4, 48), (64, 48), (48, 64)))
+    trained = [Int8Rows(r.codes, r.scales.clone().requires_grad_()) for r in (rows, w1, w2)]
+    odd = Int8Rows(w1.codes, torch.randn(128, device="cuda", requires_grad=True)[::2])
+    calls = [lambda: trained[0].values(), lambda: linear_int8(trained[0], w1), lambda: linear_int8(rows, trained[1]), lambda: linear_int8(rows, odd),
+             lambda: mlp_int8(trained[0], w1, None, w2, None), lambda: mlp_int8(rows, trained[1], None, w2, None), lambda: mlp_int8(rows, w1, None, trained[2], None)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            call()
+        with torch.no_grad():
+            assert not call().requires_grad
+    with pytest.raises(RuntimeError, match="transform"):
+        torch.func.vmap(lambda s: rows.values() * s)(torch.ones(2, device="cuda"))
