@@ -677,13 +677,19 @@ class SwinBlock(nn.Module):
         return _fused_norm_applies(feats)
 
 
-def _blocks_of(model):
-    """The Swin blocks of a network, whose widths eight bits come in."""
+def _blocks_of(model, on, most_hidden):
+    """The Swin blocks of a network.  Where they are to be switched on, eight bits have to come in their shapes: a block on which the switch
+    could never act is refused."""
     blocks = [m for m in model.modules() if isinstance(m, SwinBlock)]
-    for block in blocks:
-        widths = block.attn.dim, block.mlp.fc1.out_features
+    for block in blocks if on else ():
+        attn, widths = block.attn, (block.attn.dim, block.mlp.fc1.out_features)
         if any(w % 16 for w in widths):
             raise ValueError(f"a block of {widths[0]} channels over {widths[1]}: rows in eight bits come in multiples of 16")
+        if widths[0] > 1024 or widths[1] > most_hidden:
+            raise ValueError(f"a block of {widths[0]} channels over {widths[1]}: at most 1024 and {most_hidden}")
+        if isinstance(attn, WindowAttention) and (attn.fp16_mode not in (1, 2) or attn.head_dim not in (8, 16, 32)):
+            raise ValueError(f"a block of fp16_mode {attn.fp16_mode} and heads of {attn.head_dim} channels: eight bits are for modes 1 and 2 and heads of 8, 16 "
+                             "and 32 channels")
     return blocks
 
 
@@ -691,13 +697,11 @@ def eight_bit_inference(model, on=True):
     """Inference of the model's Swin blocks under fp16 autocast with the rows in front of their dense layers, and the layers' weights, in eight bits
     (eight_bits.py; s3d_swin_blocks_int8): a scale a row and an output channel, sums of whole numbers.  Norms, softmax, GELU and the residual stream
     stay as they are, and so do the MLPs of levels with so many voxels that both layers run as one kernel in fp16, training, and inference without
-    autocast.  Returns the model."""
-    blocks = _blocks_of(model)
-    for block in blocks:
-        widths = block.attn.dim, block.mlp.fc1.out_features
-        if widths[0] > 1024 or widths[1] > 8192:
-            raise ValueError(f"a block of {widths[0]} channels over {widths[1]}: at most 1024 and 8192 at inference")
-    for block in blocks:
+    autocast.  Returns the model.
+
+    Blocks of fp16_mode 1 and 2, heads of 8, 16 and 32 channels, widths that are multiples of 16 up to 1024 and 8192; others raise ValueError.  A block
+    whose parameters are not in fp32, or whose layers are watched or replaced, runs as without the switch."""
+    for block in _blocks_of(model, on, 8192):
         block.eight_bit_rows = bool(on)
     return model
 
@@ -705,8 +709,10 @@ def eight_bit_inference(model, on=True):
 def eight_bit_checkpoints(model, on=True):
     """Training of the model's Swin blocks under fp16 autocast with what the projection of q, k, v and the MLP read of their inputs in the backward
     pass kept in eight bits (checkpointed_linear, checkpointed_mlp): some 22 bytes a voxel and channel in place of 36.  The forward pass is the layers'
-    in fp16; gradients go by what was kept.  Inference and training without autocast stay as they are.  Returns the model."""
-    for block in _blocks_of(model):
+    in fp16; gradients go by what was kept.  Inference and training without autocast stay as they are.  Returns the model.
+
+    For the blocks that eight_bit_inference takes, the MLP's hidden layer up to 16384 channels."""
+    for block in _blocks_of(model, on, 16384):
         block.eight_bit_kept = bool(on)
     return model
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from eight_bit_reference import keep, kept, kept_scales
-from swin3d_amd import eight_bits
+from swin3d_amd import eight_bits, encoder
 from swin3d_amd.eight_bits import Int8Rows
 
 
@@ -104,3 +104,19 @@ def test_parameters_that_are_not_as_long_as_the_norm_says(name):
         assert tuple(changed.normalized_shape) == (48,)
         with pytest.raises(ValueError):
             eight_bits._norm_parameters(changed, False, 48, device)
+
+
+@pytest.mark.parametrize("switch,flag", [(encoder.eight_bit_inference, "eight_bit_rows"), (encoder.eight_bit_checkpoints, "eight_bit_kept")])
+def test_switches_refuse_blocks_on_which_they_cannot_act(switch, flag):
+    def stage(channels, heads, mode):
+        return encoder.Stage(channels, 2, heads, 5, 4, downsample=False, cRSE="XYZ_RGB", fp16_mode=mode)
+
+    for channels, heads, mode in ((48, 6, 0), (48, 12, 2), (64, 1, 1), (24, 3, 2), (48, 3, None), (1040, 65, 2)):
+        bad = stage(channels, heads, mode)
+        with pytest.raises(ValueError):
+            switch(bad)
+        assert not any(getattr(b, flag) for b in bad.blocks) and switch(bad, False) is bad
+    for channels, heads, mode in ((48, 6, 1), (48, 3, 2), (64, 2, 2)):
+        good = stage(channels, heads, mode)
+        assert switch(good) is good and all(getattr(b, flag) for b in good.blocks)
+        assert switch(good, False) is good and not any(getattr(b, flag) for b in good.blocks)
