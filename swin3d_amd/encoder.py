@@ -631,13 +631,14 @@ class SwinBlock(nn.Module):
         pending is the previous block's MLP output (or None).  The residual adds and LayerNorms run as fused
         kernels that write the normalised rows in fp16, the dtype the following GEMM reads; the block's own MLP
         output is handed on as the new pending term instead of being added here."""
+        own = pending is not None      # (the sum is a tensor of this call)
         if self.eight_bit_rows:
-            whole = feats if pending is None else _plus(feats, pending)
-            done = swin_blocks(self, [self], (SwinBlock, WindowAttention, Mlp), whole, [attn_args], _cache_epoch(), None, eight_bits=True)
+            feats, pending = (_plus(feats, pending), None) if own else (feats, None)
+            done = swin_blocks(self, [self], (SwinBlock, WindowAttention, Mlp), feats, [attn_args], _cache_epoch(), None, eight_bits=True)
             if done is not None:
                 return done
         feats, normed = add_layernorm(feats, pending, self.norm1)
-        feats, normed = add_layernorm(feats, self.attn(normed, attn_args), self.norm2, inplace=pending is not None)
+        feats, normed = add_layernorm(feats, self.attn(normed, attn_args), self.norm2, inplace=own)
         return feats, self.mlp(normed)
 
     def forward_trained(self, feats, pending, attn_args):

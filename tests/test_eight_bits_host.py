@@ -120,3 +120,27 @@ def test_switches_refuse_blocks_on_which_they_cannot_act(switch, flag):
         good = stage(channels, heads, mode)
         assert switch(good) is good and all(getattr(b, flag) for b in good.blocks)
         assert switch(good, False) is good and not any(getattr(b, flag) for b in good.blocks)
+
+
+def test_a_block_adds_what_is_pending_once(monkeypatch):
+    """Where the call in eight bits does not apply, the sum that was made for it is the stream of the layers one by one."""
+    calls = []
+    monkeypatch.setattr(encoder, "swin_blocks", lambda *_, **__: None)
+
+    def add_layernorm(x, residual, norm, inplace=False):
+        calls.append((residual is not None, inplace))
+        summed = x if residual is None else x + residual
+        return summed, norm(summed)
+
+    monkeypatch.setattr(encoder, "add_layernorm", add_layernorm)
+    block = encoder.SwinBlock(48, 6, 5, 4, fp16_mode=2)
+    monkeypatch.setattr(block.attn, "forward", lambda x, args: 2 * x)
+    feats, pending = torch.randn(4, 48), torch.randn(4, 48)
+    with torch.no_grad():
+        want, want_at_first = block.forward_fused(feats, pending, None), block.forward_fused(feats, None, None)
+        assert calls == [(True, False), (True, True), (False, False), (True, False)]
+        encoder.eight_bit_inference(block)
+        calls.clear()
+        got, got_at_first = block.forward_fused(feats, pending, None), block.forward_fused(feats, None, None)
+    assert calls == [(False, False), (True, True), (False, False), (True, False)]
+    assert all(torch.equal(a, b) for a, b in zip(got + got_at_first, want + want_at_first))

@@ -215,3 +215,22 @@ def test_a_network_with_both(hip_lib):
         got = model(voxels, signals)
         want = eight_bit_inference(model, False)(voxels, signals)
     assert got.isfinite().all() and not torch.equal(got, want) and float((got - want).norm() / want.norm()) < 0.05
+
+
+def test_blocks_that_cannot_any_more_are_what_they_were(hip_lib):
+    """A block that turns to fp16_mode 0 behind the switch runs as without it, to the bit, among others and by itself, and leaves its input alone."""
+    stage, coords, signals, feats = _stage(6, 8, 5, 2, 3000)
+    stage.eval()
+    with torch.no_grad():
+        plan = stage.plan(coords, 1, signals)
+        for changed in ([0, 1, 2], [1]):
+            eight_bit_inference(stage)
+            for i in changed:
+                stage.blocks[i].attn.fp16_mode = 0
+            given, got = feats.clone(), _run(stage, coords, signals, feats, plan)
+            assert torch.equal(feats, given)
+            for i in changed:
+                stage.blocks[i].eight_bit_rows = False
+            assert torch.equal(_run(stage, coords, signals, feats, plan), got)
+            for block in stage.blocks:
+                block.attn.fp16_mode = 2
