@@ -8,6 +8,7 @@ from torch.autograd import forward_ad
 from torch.nn.modules import module as _module_hooks
 
 from . import _lib
+from .crse import crse_num_axes
 from .sparse_dl.attn import attn_coff
 
 
@@ -136,6 +137,19 @@ def _eight_bit_descriptions(parts):
     return blocks, kept
 
 
+def _sized(m, weight, bias):
+    """The parameters of a layer are of these shapes (its bias may be None).  Its attributes do not say so: a program may have put other
+    parameters in their place, and the library reads as many numbers as it is told."""
+    w, b = m._parameters.get("weight"), m._parameters.get("bias")
+    return w is not None and w.shape == weight and (b is None or b.shape == bias)
+
+
+def _whole_tables(parts):
+    """The tables of every block are as long as its table_sizes say."""
+    return all(sum(getattr(attn, f"{kind}_{name}_table").numel() for name in ("xyz", "rgb", "norm")[:crse_num_axes(attn.cRSE) // 3]) == sum(attn.table_sizes)
+               for _, _, attn, *_ in parts for kind in ("query", "key", "value"))
+
+
 def _applicable(parts, channels):
     attn, fc1 = parts[0][2], parts[0][7]
     if attn.fp16_mode not in (1, 2) or attn.head_dim not in (8, 16, 32) or channels % 16 or fc1.out_features % 16:
@@ -145,11 +159,11 @@ def _applicable(parts, channels):
                 or list(a.table_sizes) != list(attn.table_sizes):
             return False
         for norm in (norm1, norm2):
-            if tuple(norm.normalized_shape) != (channels,) or norm.weight is None or norm.bias is None:
+            if tuple(norm.normalized_shape) != (channels,) or norm.bias is None or not _sized(norm, (channels,), (channels,)):
                 return False
         shapes = [(qkv, channels, 3 * channels), (proj, channels, channels), (f1, channels, fc1.out_features),
                   (f2, fc1.out_features, channels)]
-        if any((m.in_features, m.out_features) != (i, o) for m, i, o in shapes):
+        if any((m.in_features, m.out_features) != (i, o) or not _sized(m, (o, i), (o,)) for m, i, o in shapes):
             return False
         # the fp16 copies of fp32 parameters on one device
         if any(p.dtype != torch.float32 or p.device != qkv.weight.device
@@ -201,7 +215,7 @@ def swin_blocks(owner, blocks, kinds, feats, index_sets, epoch, half_copy, eight
     kept = None if captured else getattr(owner, "_s3d_blocks", None)
     if kept is None or kept.key != key:
         describe = _eight_bit_descriptions if eight_bits else lambda parts: _descriptions(parts, half_copy)
-        kept = _Kept(key, *(describe(parts) if _applicable(parts, channels) else (None, None)))
+        kept = _Kept(key, *(describe(parts) if _applicable(parts, channels) and _whole_tables(parts) else (None, None)))
         if not captured:
             owner._s3d_blocks = kept
     if kept.described is None:

@@ -77,3 +77,37 @@ def test_a_scale_set_after_a_call_reaches_the_projection():
         attn.scale *= 2
         second = attn._prepared()[0]
     assert torch.equal(second[:16], 2 * first[:16]) and torch.equal(second[16:], first[16:])
+
+
+def _other(shape):
+    return nn.Parameter(torch.zeros(shape))
+
+
+@pytest.mark.parametrize("layer,name,shape", [
+    ("mlp.fc1", "weight", (48, 16)), ("mlp.fc1", "bias", (48,)), ("mlp.fc2", "weight", (16, 48)), ("mlp.fc2", "bias", (1,)), ("attn.qkv", "weight", (32, 16)),
+    ("attn.qkv", "bias", (16,)), ("attn.proj", "weight", (16, 8)), ("norm1", "weight", (8,)), ("norm1", "bias", (0,)), ("norm2", "weight", (0,)),
+    ("norm2", "bias", (32,)),
+])
+def test_parameters_of_other_sizes_than_the_layers_say(layer, name, shape):
+    """The library reads by the layers' sizes: a block whose parameters are no longer of them runs layer by layer."""
+    block = encoder.SwinBlock(16, 2, 5, 4, cRSE="XYZ_RGB", fp16_mode=2)
+    parts = swin_blocks._parts(block, (encoder.SwinBlock, encoder.WindowAttention, encoder.Mlp))
+    assert swin_blocks._applicable([parts], 16)
+    setattr(block.get_submodule(layer), name, _other(shape))
+    assert not swin_blocks._applicable([parts], 16)
+
+
+def test_layers_without_biases_are_of_their_sizes():
+    block = encoder.SwinBlock(16, 2, 5, 4, cRSE="XYZ_RGB", fp16_mode=2)
+    for layer in (block.attn.qkv, block.attn.proj, block.mlp.fc1, block.mlp.fc2):
+        layer.bias = None
+    assert swin_blocks._applicable([swin_blocks._parts(block, (encoder.SwinBlock, encoder.WindowAttention, encoder.Mlp))], 16)
+
+
+@pytest.mark.parametrize("cRSE", ["XYZ", "XYZ_RGB", "XYZ_RGB_NORM"])
+def test_tables_of_other_lengths_than_their_sizes_say(cRSE):
+    block = encoder.SwinBlock(16, 2, 5, 4, cRSE=cRSE, fp16_mode=2)
+    parts = [swin_blocks._parts(block, (encoder.SwinBlock, encoder.WindowAttention, encoder.Mlp))]
+    assert swin_blocks._whole_tables(parts)
+    block.attn.key_xyz_table = _other((3, 39, 2, 8))
+    assert not swin_blocks._whole_tables(parts)
