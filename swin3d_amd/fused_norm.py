@@ -23,6 +23,9 @@ def add_layernorm(x, residual, norm, out_dtype=torch.float16, inplace=False):
     n, c = x.shape
     if tuple(norm.normalized_shape) != (c,) or norm.weight is None or norm.bias is None:
         raise ValueError("norm must be an affine LayerNorm over the channel axis")
+    if not norm.weight.shape == norm.bias.shape == (c,) or not norm.weight.device == norm.bias.device == x.device:
+        raise ValueError(f"norm's parameters must be [{c}] on {x.device}, got {tuple(norm.weight.shape)} on {norm.weight.device} and "
+                         f"{tuple(norm.bias.shape)} on {norm.bias.device}")
     if out_dtype not in _DTYPE_CODE:
         raise ValueError(f"out_dtype {out_dtype} (float16 or float32)")
     x = x.contiguous()
@@ -142,6 +145,7 @@ def trained_add_norm(x, residual, norm):
         return None
     weight, bias = norm.weight, norm.bias
     if weight is None or bias is None or x.dim() != 2 or x.shape[0] == 0 or tuple(norm.normalized_shape) != (x.shape[1],) \
+            or not weight.shape == bias.shape == x.shape[1:] \
             or x.shape[1] % 4 or x.shape[1] > 1024:
         return None
     for t, dtype in ((x, torch.float32), (weight, torch.float32), (bias, torch.float32), (residual, torch.float16)):

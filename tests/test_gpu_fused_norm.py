@@ -139,3 +139,28 @@ def test_sum_with_a_branch_in_fp16(hip_lib, rows, channels):
     assert add_half(x, branch.float()) is None
     if rows > 1:
         assert add_half(x.t(), branch.t()) is None and add_half(x[:, :3], branch[:, :3]) is None
+
+
+@pytest.mark.parametrize("name", ["weight", "bias"])
+@pytest.mark.parametrize("size", [0, 44, 96])
+def test_norms_whose_parameters_are_not_as_long_as_they_say(hip_lib, name, size):
+    """normalized_shape is a plain attribute: the kernels read a number a channel of each parameter."""
+    from swin3d_amd.fused_norm import add_layernorm, trained_add_norm
+    norm, x = torch.nn.LayerNorm(48, device="cuda"), torch.randn(8, 48, device="cuda")
+    getattr(norm, name).data = torch.ones(size, device="cuda")
+    with torch.no_grad(), pytest.raises(ValueError):
+        add_layernorm(x, None, norm)
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert trained_add_norm(x.requires_grad_(), None, norm) is None
+    with torch.no_grad(), pytest.raises(ValueError):
+        add_layernorm(x.detach(), None, torch.nn.LayerNorm(48))
+
+
+def test_block_whose_norm_is_not_as_long_as_it_says(hip_lib):
+    """Neither the calls by address nor the layers one by one read behind it."""
+    from swin3d_amd import encoder
+    for training in (False, True):
+        block = encoder.SwinBlock(48, 6, 5, 4, cRSE="XYZ_RGB", fp16_mode=2).cuda()
+        block.norm1.weight.data = torch.ones(44, device="cuda")
+        with torch.set_grad_enabled(training), torch.autocast("cuda", dtype=torch.float16), pytest.raises((ValueError, RuntimeError)):
+            block(torch.randn(8, 48, device="cuda"), (None,) * 9)
