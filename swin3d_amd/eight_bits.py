@@ -58,7 +58,10 @@ class Int8Rows(NamedTuple):
 
 
 def _dense(t):
-    """t as the kernels read it: dense and 16-byte aligned."""
+    """t as the kernels read it: dense and 16-byte aligned.  (A parameter whose storage has been freed has a null pointer, which of a bias, a norm's weight or
+    a residual would say that there is none.)"""
+    if t.data_ptr() == 0 and t.numel() > 0:
+        raise ValueError(f"a tensor {tuple(t.shape)} without memory")
     t = t if t.is_contiguous() else t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -97,7 +100,7 @@ _ANY_ROWS = (None, None)
 
 def _ready(dev, *tensors):
     """All of them (None aside) are plain, dense and 16-byte aligned on `dev`: nothing about them has to be looked at or copied but shapes and types."""
-    return all(t is None or (type(t) in _PLAIN and t.device == dev and t.is_contiguous() and t.data_ptr() % 16 == 0) for t in tensors)
+    return all(t is None or (type(t) in _PLAIN and t.device == dev and t.is_contiguous() and (at := t.data_ptr()) != 0 and at % 16 == 0) for t in tensors)
 
 
 _PLAIN = (torch.Tensor, nn.Parameter)
@@ -153,7 +156,7 @@ def add_norm_int8(x, residual, norm, inplace=False):
         residual = _dense(residual)
         res_ptr, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]
         summed = x if inplace else torch.empty((n, c), dtype=torch.float32, device=dev)
-    gamma, beta = (None if p is None else _dense(p if p.dtype is torch.float32 else p.detach().float()) for p in (weight, bias))
+    gamma, beta = (None if p is None else _dense(p) if p.dtype is torch.float32 else _dense(p).detach().float() for p in (weight, bias))
     rows = _empty_rows(n, c, dev)
     with _lib.on(dev):
         status = _lib.lib().s3d_add_norm_int8(
@@ -189,7 +192,7 @@ def _layer_operands(name, weight, bias, k, dev):
         raise ValueError(f"{name} takes {codes.shape[1]} channels, the rows have {k}")
     if bias is not None:
         _check(f"the bias of {name}", bias, (torch.float32, torch.float16), (n,), dev)
-        bias = _dense(bias.float())      # (where autograd follows it, the result requires a gradient and is refused)
+        bias = _dense(bias).float()      # (where autograd follows it, the result requires a gradient and is refused)
     return _dense(codes), _dense(scales), bias
 
 

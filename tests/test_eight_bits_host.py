@@ -144,3 +144,16 @@ def test_a_block_adds_what_is_pending_once(monkeypatch):
         got, got_at_first = block.forward_fused(feats, pending, None), block.forward_fused(feats, None, None)
     assert calls == [(False, False), (True, True), (False, False), (True, False)]
     assert all(torch.equal(a, b) for a, b in zip(got + got_at_first, want + want_at_first))
+
+
+def test_tensors_whose_storage_was_freed():
+    for shape in ((48,), (4, 48)):
+        t = torch.zeros(shape)
+        assert eight_bits._ready(t.device, t) and eight_bits._dense(t) is t
+        strided = t[..., ::2]
+        t.untyped_storage().resize_(0)
+        assert not eight_bits._ready(t.device, t)
+        for view in (t, strided):
+            with pytest.raises(ValueError, match="without memory"):
+                eight_bits._dense(view)
+    assert eight_bits._dense(torch.zeros(0, 48)).shape == (0, 48)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from eight_bit_reference import gelu, int8_rows
-from swin3d_amd.eight_bits import Int8Rows, add_norm_int8, linear_int8, mlp_int8, quantize_rows
+from swin3d_amd.eight_bits import Int8Rows, add_norm_int8, checkpointed_linear, checkpointed_mlp, linear_int8, mlp_int8, quantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -372,3 +372,24 @@ def test_scales_that_require_a_gradient(hip_lib):
             assert not call().requires_grad
     with pytest.raises(RuntimeError, match="transform"):
         torch.func.vmap(lambda s: rows.values() * s)(torch.ones(2, device="cuda"))
+
+
+def test_operands_whose_storage_was_freed(hip_lib):
+    """Their null pointers are no sign that there is no bias, weight or residual."""
+    def freed(*shape, dtype=torch.float32):
+        t = torch.zeros(shape, device="cuda", dtype=dtype)
+        t.untyped_storage().resize_(0)
+        return t
+
+    x, norm = torch.randn(4, 48, device="cuda"), torch.nn.LayerNorm(48, device="cuda").requires_grad_(False)
+    rows, w1, w2 = (quantize_rows(torch.randn(n, k, device="cuda")) for n, k in ((4, 48), (64, 48), (48, 64)))
+    emptied = [torch.nn.LayerNorm(48, device="cuda").requires_grad_(False) for _ in range(2)]
+    emptied[0].weight.data, emptied[1].bias.data = freed(48), freed(48)
+    half, w = x.half(), torch.randn(64, 48, device="cuda")
+    for call in (lambda: add_norm_int8(x, freed(4, 48), norm), lambda: add_norm_int8(x, None, emptied[0]), lambda: add_norm_int8(x, None, emptied[1]),
+                 lambda: linear_int8(rows, w1, freed(64)), lambda: linear_int8(rows, w1, freed(64, dtype=torch.float16)), lambda: linear_int8(Int8Rows(rows.codes, freed(4)), w1),
+                 lambda: mlp_int8(rows, w1, freed(64), w2, None), lambda: mlp_int8(rows, w1, None, w2, freed(48)), lambda: quantize_rows(freed(4, 48)),
+                 lambda: checkpointed_linear(half, w, freed(64)), lambda: checkpointed_linear(half, freed(64, 48), None),
+                 lambda: checkpointed_mlp(half, w, freed(64), w.t().contiguous(), None), lambda: checkpointed_mlp(half, w, None, w.t().contiguous(), freed(48))):
+        with pytest.raises(ValueError, match="without memory"):
+            call()
