@@ -141,7 +141,9 @@ def add_norm_int8(x, residual, norm, inplace=False):
     if c == 0 or c % 4 or c > _MOST_CHANNELS:
         raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
     rms = isinstance(norm, nn.RMSNorm)
-    if not (rms or isinstance(norm, nn.LayerNorm)) or tuple(norm.normalized_shape) != (c,):
+    kind = nn.RMSNorm if rms else nn.LayerNorm
+    # (a class or an instance with a forward of its own is another norm)
+    if not isinstance(norm, kind) or type(norm).forward is not kind.forward or "forward" in norm.__dict__ or tuple(norm.normalized_shape) != (c,):
         raise ValueError(f"norm must be a LayerNorm or RMSNorm over the {c} channels, got {norm}")
     weight, bias = _norm_parameters(norm, rms, c, dev)
     if residual is not None:

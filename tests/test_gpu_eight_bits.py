@@ -393,3 +393,23 @@ def test_operands_whose_storage_was_freed(hip_lib):
                  lambda: checkpointed_mlp(half, w, freed(64), w.t().contiguous(), None), lambda: checkpointed_mlp(half, w, None, w.t().contiguous(), freed(48))):
         with pytest.raises(ValueError, match="without memory"):
             call()
+
+
+@pytest.mark.parametrize("kind", [torch.nn.LayerNorm, torch.nn.RMSNorm])
+def test_norms_with_a_forward_of_their_own(hip_lib, kind):
+    """Such as add one to their weight: other norms, which the kernel does not know.  A class that only adds to the parameters is the same norm."""
+    class Other(kind):
+        def forward(self, x):
+            return super().forward(x) + x
+
+    class Same(kind):
+        def extra_repr(self):
+            return "same"
+
+    x = torch.randn(4, 48, device="cuda")
+    norms = [cls(48, device="cuda").requires_grad_(False) for cls in (Other, kind, Same, kind)]
+    norms[1].forward = lambda x: x
+    for norm in norms[:2]:
+        with pytest.raises(ValueError, match="must be a LayerNorm or RMSNorm"):
+            add_norm_int8(x, None, norm)
+    assert all(torch.equal(a, b) for a, b in zip(add_norm_int8(x, None, norms[2])[1], add_norm_int8(x, None, norms[3])[1]))
