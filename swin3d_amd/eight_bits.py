@@ -165,6 +165,8 @@ def add_norm_int8(x, residual, norm, inplace=False):
             rows_in.data_ptr(), res_ptr, res_code, None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), float(eps),
             int(rms), None if residual is None else summed.data_ptr(), rows.codes.data_ptr(), rows.scales.data_ptr(), n, c, _lib.stream(dev))
     _lib.check(status, "s3d_add_norm_int8")
+    if residual is not None and inplace:
+        torch.autograd.graph.increment_version(x)      # (as torch's own changes in place: a graph that has kept x for its backward refuses it then)
     return summed, rows
 
 

@@ -45,6 +45,8 @@ def add_layernorm(x, residual, norm, out_dtype=torch.float16, inplace=False):
                                              float(norm.eps), summed.data_ptr() if residual is not None else None,
                                              y.data_ptr(), _DTYPE_CODE[out_dtype], n, c, stream)
     _lib.check(status, "s3d_add_layernorm")
+    if residual is not None and inplace:
+        torch.autograd.graph.increment_version(x)      # (as torch's own changes in place: a graph that has kept x for its backward refuses it then)
     return summed, y
 
 

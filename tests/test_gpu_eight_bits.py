@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from eight_bit_reference import gelu, int8_rows
+from swin3d_amd import add_layernorm
 from swin3d_amd.eight_bits import Int8Rows, add_norm_int8, checkpointed_linear, checkpointed_mlp, linear_int8, mlp_int8, quantize_rows
 
 pytestmark = pytest.mark.gpu
@@ -413,3 +414,23 @@ def test_norms_with_a_forward_of_their_own(hip_lib, kind):
         with pytest.raises(ValueError, match="must be a LayerNorm or RMSNorm"):
             add_norm_int8(x, None, norm)
     assert all(torch.equal(a, b) for a, b in zip(add_norm_int8(x, None, norms[2])[1], add_norm_int8(x, None, norms[3])[1]))
+
+
+@pytest.mark.parametrize("call", [add_norm_int8, add_layernorm])
+def test_sum_in_place_is_a_change_that_autograd_sees(hip_lib, call):
+    """A graph that has kept x for its backward would compute from the sum otherwise."""
+    norm = torch.nn.LayerNorm(48, device="cuda").requires_grad_(False)
+    x, residual, w = torch.randn(4, 48, device="cuda"), torch.randn(4, 48, device="cuda"), torch.randn(48, 8, device="cuda", requires_grad=True)
+    for inplace, given in ((False, residual), (True, None), (True, residual)):
+        y, version = x @ w, x._version
+        with torch.no_grad():
+            summed, _ = call(x, given, norm, inplace=inplace)
+        changed = inplace and given is not None
+        assert (summed is x) == (given is None or inplace) and (x._version > version) == changed
+        if not changed:
+            y.sum().backward()
+            continue
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        call(torch.randn(4, 48, device="cuda"), residual, norm, inplace=True)
