@@ -465,9 +465,11 @@ def checkpointed_linear(x, weight, bias=None, scaled=None):
     _check_layer("weight", weight, bias, x.shape[1], x.device)
     _no_followers("checkpointed_linear")
     rows, factor = (0, 1.0) if scaled is None else scaled
-    if not 0 <= rows <= weight.shape[0] or rows % 16:
+    if not hasattr(type(rows), "__index__") or isinstance(rows, torch.Tensor) or not 0 <= rows <= weight.shape[0] or rows % 16:
         raise ValueError(f"{rows} scaled outputs of {weight.shape[0]} (a multiple of 16)")
-    return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias, (rows, float(factor)))
+    if isinstance(factor, torch.Tensor) and factor.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the factor of scaled outputs is a number, of which there is no gradient: multiply the parameters where it is trained")
+    return _KeptLinear.apply(torch.is_grad_enabled(), x, weight, bias, (int(rows), float(factor)))
 
 
 def checkpointed_mlp(x, weight1, bias1, weight2, bias2):

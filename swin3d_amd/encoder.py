@@ -650,7 +650,8 @@ class SwinBlock(nn.Module):
             return None
         if self.eight_bit_kept:
             parts = _parts(self, (SwinBlock, WindowAttention, Mlp))
-            if parts is not None and _applicable([parts], feats.shape[1]):
+            # (a scale that is a tensor may be trained: the layers one by one have its gradient)
+            if parts is not None and _applicable([parts], feats.shape[1]) and not isinstance(self.attn.scale, torch.Tensor):
                 return self._trained_in_eight_bits(*done, attn_args)
         whole = trained_branches(self, (SwinBlock, WindowAttention, Mlp), *done, attn_args)
         if whole is not None:

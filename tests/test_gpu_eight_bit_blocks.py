@@ -234,3 +234,16 @@ def test_blocks_that_cannot_any_more_are_what_they_were(hip_lib):
             assert torch.equal(_run(stage, coords, signals, feats, plan), got)
             for block in stage.blocks:
                 block.attn.fp16_mode = 2
+
+
+def test_scale_that_is_trained(hip_lib):
+    """A block whose attention's scale is a tensor has its gradient, with the switch as without."""
+    stage, coords, signals, feats = _stage(6, 8, 5, 1, 3000, depth=1)
+    plan, attn, given = stage.plan(coords, 1, signals), stage.blocks[0].attn, []
+    for on in (False, True):
+        eight_bit_checkpoints(stage, on)
+        attn.scale = torch.tensor(8 ** -0.5, device="cuda", requires_grad=True)
+        out = _run(stage, coords, signals, feats, plan)
+        grad, = torch.autograd.grad(out.square().sum(), attn.scale)
+        given.append((out.detach(), grad))
+    assert all(torch.equal(a, b) for a, b in zip(*given)) and float(given[0][1].abs()) > 0

@@ -444,3 +444,19 @@ def test_form_of_more_than_32_bits_of_bytes(hip_lib):
     assert torch.equal(got[(m - last) * c:m * c], tail[:last * c]) and torch.equal(got[-last * (c // GROUP):], tail[last * c:])
     values = kept_values(got, c)
     assert values.shape == x.shape and torch.equal(values[-last:], kept_values(tail, c)) and not values[:-last].any()
+
+
+def test_factor_that_is_trained(hip_lib):
+    """The factor of scaled outputs is a number: one that requires a gradient is refused, not dropped."""
+    import numpy as np
+    x, w = torch.randn(4, 32, device="cuda").half(), torch.randn(48, 32, device="cuda", requires_grad=True)
+    factor = torch.tensor(0.5, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        checkpointed_linear(x, w, None, (16, factor))
+    want = checkpointed_linear(x, w, None, (16, 0.5))
+    with torch.no_grad():
+        assert torch.equal(checkpointed_linear(x, w, None, (16, factor)), want)
+    assert torch.equal(checkpointed_linear(x, w, None, (np.int64(16), factor.detach())), want)
+    for rows in (16.0, torch.tensor(16), "16", None):
+        with pytest.raises(ValueError):
+            checkpointed_linear(x, w, None, (rows, 0.5))
