@@ -8,8 +8,9 @@ channel, and the product a sum of whole numbers, exact, with both scales behind 
     y = mlp_int8(rows, quantize_rows(fc1.weight), fc1.bias, quantize_rows(fc2.weight), fc2.bias)
 
 In training a layer keeps what its backward reads of its input in eight bits, in groups of sixteen numbers with a scale each
-(`keep_rows`): the forward is the layer's own in fp16, and so is the gradient of its input; the weight's gradient is that of rows a 254th of
-their group's largest number off at most, and an eighth of that more where a scale of four bits is above what the group needs:
+(`keep_rows`): the forward is the layer's own in fp16, and so is the gradient of its input; the weight's gradient is that of rows half a step off at most.
+That is a 254th of their group's largest number, and where a scale of four bits is above what the group needs up to an eighth of that more; in groups whose
+largest number is below 127 2^-21, whose scales are whole multiples of 2^-24, up to 2^-25 more; and of numbers above 65,088, where codes end, up to 416:
 
     y = checkpointed_linear(x, layer.weight, layer.bias)
     y = checkpointed_mlp(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias)

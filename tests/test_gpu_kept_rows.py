@@ -460,3 +460,24 @@ def test_factor_that_is_trained(hip_lib):
     for rows in (16.0, torch.tensor(16), "16", None):
         with pytest.raises(ValueError):
             checkpointed_linear(x, w, None, (rows, 0.5))
+
+
+def test_how_far_the_form_is_off_at_both_ends(hip_lib):
+    """Every fp16 size as its group's largest number, beside numbers below it.  A scale s is the smallest of four bits, and of whole 2^-24, that reaches the
+    largest number a with 127 codes: s <= 1.125 a / 127 from 8 2^-24 on, less than a / 127 + 2^-24 below, and a number is off by s / 2 at most.  Above 127 512
+    = 65,024 s is 576 and codes end at 113, for 65,088: up to 65,504 is 416 off."""
+    sizes = torch.arange(0, 0x7c00, dtype=torch.int16, device="cuda").view(torch.float16)
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = (sizes.float().unsqueeze(1) * torch.rand(sizes.numel(), GROUP, device="cuda", generator=gen)).half()
+    x[:, 0], x[:, 1] = sizes, -sizes
+    x = torch.minimum(x, sizes.unsqueeze(1))
+    off = (kept_values(keep_rows(x), GROUP).double() - x.double()).abs()
+    most = x.double().abs().amax(1, keepdim=True)
+    assert torch.equal(most[:, 0], sizes.double())
+    unit = 2.0 ** -24
+    bound = 0.5 * torch.where(most > 127 * 8 * unit, 1.125 * most / 127, most / 127 + unit)
+    top = most > 65024
+    assert int(top.sum()) == 15 and bool((off <= torch.where(top, 416.0, bound)).all())
+    assert float(off[top[:, 0]].max()) == 416 and float((off / bound)[~top[:, 0]].max()) > 0.85
+    small = (most[:, 0] > 127 * unit) & (most[:, 0] < 254 * unit)      # ... where the scale is a whole 2^-24: up to twice a 254th
+    assert float((off / (most / 254))[small].max()) > 1.5
