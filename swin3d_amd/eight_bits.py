@@ -61,10 +61,12 @@ class Int8Rows(NamedTuple):
 def _dense(t):
     """t as the kernels read it: dense and 16-byte aligned.  (A parameter whose storage has been freed has a null pointer, which of a bias, a norm's weight or
     a residual would say that there is none.)"""
-    if t.data_ptr() == 0 and t.numel() > 0:
+    at = t.data_ptr()
+    if at == 0 and t.numel() > 0:
         raise ValueError(f"a tensor {tuple(t.shape)} without memory")
-    t = t if t.is_contiguous() else t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if at % 16 == 0 else t.clone()
 
 
 def _check(name, t, dtypes, shape, device=None):
