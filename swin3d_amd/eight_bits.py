@@ -42,15 +42,18 @@ class Int8Rows(NamedTuple):
 
     def values(self, dtype=torch.float16):
         """[N,C] in float16 or float32: what the rows stand for.  No autograd."""
-        _check_rows("rows", self)
+        codes, scales = self
+        if not (isinstance(codes, torch.Tensor) and codes.is_cuda and scales is not None and _ready(codes.device, codes, scales) and codes.dtype is torch.int8 and codes.dim() == 2
+                and scales.dtype is torch.float32 and scales.shape == codes.shape[:1] and codes.shape[0] <= 0x7fffffff):
+            _check_rows("rows", self)
+            codes, scales = _dense(codes), _dense(scales)
         if dtype not in _DTYPE_CODE:
             raise ValueError(f"dtype {dtype} (float16 or float32)")
-        n, c = self.codes.shape
+        n, c = codes.shape
         if c == 0 or c % 4 or c > _MOST_CHANNELS:
             raise ValueError(f"rows of {c} channels (a multiple of 4, at most {_MOST_CHANNELS})")
-        _unfollowed("Int8Rows.values", self.scales)
-        dev = self.codes.device
-        codes, scales = _dense(self.codes), _dense(self.scales)
+        _unfollowed("Int8Rows.values", scales)
+        dev = codes.device
         out = torch.empty((n, c), dtype=dtype, device=dev)
         with _lib.on(dev):
             status = _lib.lib().s3d_int8_values(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), _DTYPE_CODE[dtype], n, c, _lib.stream(dev))
@@ -113,8 +116,10 @@ def _unfollowed(what, *tensors):
     """These calls are no operations of autograd: nothing may follow them."""
     if followed():
         raise RuntimeError(f"{what} does not run under a transform, a forward-mode derivative, a dispatch mode or a tracer")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach what requires one")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach what requires one")
 
 
 def _empty_rows(n, c, device):
@@ -126,7 +131,7 @@ def _norm_parameters(norm, rms, c, dev):
     are by now: the kernel reads c numbers of each."""
     weight, bias = norm.weight, None if rms else norm.bias
     for name, p in (("norm.weight", weight), ("norm.bias", bias)):
-        if p is not None and not (p.dtype is torch.float32 and p.device == dev and p.shape == (c,)):
+        if p is not None and not (p.dtype is torch.float32 and p.device == dev and p.dim() == 1 and p.numel() == c):
             _check(name, p, (torch.float32, torch.float16, torch.bfloat16, torch.float64), (c,), dev)
     return weight, bias
 
