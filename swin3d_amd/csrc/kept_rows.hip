@@ -356,10 +356,11 @@ extern "C" __attribute__((visibility("default"))) int s3d_kept_mlp_grad(const vo
             const KeptMlp a{dy, w2_t, nullptr, w1_t, nullptr, dx, nullptr, const_cast<void *>(kept_h), dhidden, active, sums, M, C, hidden};
             if (int rc = launch_kept_mlp_grad(a, s)) return rc;
         } else {
-            LinearArgs a{dy, w2_t, sums, dhidden, M, hidden, C, false};
+            LinearArgs a{dy, w2_t, nullptr, dhidden, M, hidden, C, false};
             a.kept_grad = true;
-            a.kept = kept_h;
+            a.kept = const_cast<void *>(kept_h);
             a.gelu_out = active;
+            a.sums = sums;
             if (int rc = launch_linear(a, s)) return rc;
             if (dx)
                 if (int rc = launch_linear({dhidden, w1_t, nullptr, dx, M, C, hidden, false}, s)) return rc;

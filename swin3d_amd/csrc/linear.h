@@ -14,11 +14,12 @@ struct LinearArgs {
     const void *gelu_at = nullptr;   // [M,N] fp16: the rows, rounded, are gradients behind a GELU of these, and y those before it
     bool in_order = false;           // a number's K products are added up one after the other, whatever the tile
     void *gelu_out = nullptr;        // [M,N] fp16: GELU of y's rounded rows, beside them (in_order; without gelu and gelu_at)
-    // Rows in eight bits (rows8.h; without gelu, gelu_at and in_order, N a multiple of 16).  keep: in place of y the rounded rows go there
-    // (unless kept is null) and GELU of them to gelu_out.  kept_grad: the rows are gradients behind a GELU of what is kept there, y those
-    // before it, and gelu_out GELU of what is kept.
+    // Rows in eight bits (rows8.h; without gelu, gelu_at and in_order, N a multiple of 16).  keep: in place of y the rounded rows go to kept
+    // (unless it is null) and GELU of them to gelu_out.  kept_grad: the rows are gradients behind a GELU of what kept has, y those before it,
+    // gelu_out GELU of what is kept, and sums the results added up over each 32 rows before they are rounded; no bias.
     bool keep = false, kept_grad = false;
-    const void *kept = nullptr;
+    void *kept = nullptr;            // written by keep, read by kept_grad
+    float *sums = nullptr;           // [ceil(M / 32)][N]
 };
 
 int launch_linear(const LinearArgs &a, hipStream_t stream);

@@ -30,8 +30,9 @@ static_assert(kChunk / 8 == kPieces, "pieces of eight numbers");
 __device__ __forceinline__ float gelu_erf(float x) { return (x * 0.5f) * (1.0f + erff(x * 0.70710678f)); }
 
 // The last two are of layers that keep rows in eight bits (kept_rows.hip), in `gelu_at`'s place: kKeep leaves the rows' codes and GELU of
-// the rows, rounded, in `gelu_out`; kKeptGrad multiplies by GELU's slope at what was kept, in fp32, and leaves GELU of that in `gelu_out` and,
-// where `bias` points, the results' sums over each 32 rows before they are rounded, fp32 [ceil(M / 32)][N].
+// the rows, rounded, in `gelu_out`; kKeptGrad multiplies by GELU's slope at what was kept, in fp32, and leaves GELU of that in `gelu_out` and, in
+// `bias`'s place, which it has none of, the results' sums over each 32 rows before they are rounded, fp32 [ceil(M / 32)][N].  (Arguments of their own
+// would be two more of every product's.)
 enum class Behind { kNothing, kGelu, kGeluGrad, kGeluBeside, kKeep, kKeptGrad };
 
 // WM x WN wavefronts of TM x TN products of 32 x 32
@@ -302,9 +303,10 @@ int launch(const LinearArgs &a, hipStream_t stream)
     constexpr int kPerCu = 160 * 1024 / L::kLds < 2 ? 1 : 160 * 1024 / L::kLds < 4 ? 160 * 1024 / L::kLds : 4;
     const int64_t slots = static_cast<int64_t>(kPerCu) * device_cus();
     const dim3 grid(static_cast<unsigned>(ceil_div(tiles < slots ? tiles : slots, 8) * 8));
+    const void *bias = a.kept_grad ? a.sums : a.bias, *gelu_at = a.keep || a.kept_grad ? a.kept : a.gelu_at;
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, static_cast<const _Float16 *>(a.x), static_cast<const _Float16 *>(a.w),
-                       static_cast<const _Float16 *>(a.bias), static_cast<_Float16 *>(a.y),
-                       static_cast<const _Float16 *>(a.keep || a.kept_grad ? a.kept : a.gelu_at), static_cast<_Float16 *>(a.gelu_out), static_cast<int>(a.M), a.N, a.K, tiles_n, static_cast<int>(tiles));
+                       static_cast<const _Float16 *>(bias), static_cast<_Float16 *>(a.y), static_cast<const _Float16 *>(gelu_at),
+                       static_cast<_Float16 *>(a.gelu_out), static_cast<int>(a.M), a.N, a.K, tiles_n, static_cast<int>(tiles));
     S3D_HIP_CHECK(hipGetLastError());
     return S3D_OK;
 }
