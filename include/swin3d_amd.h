@@ -728,7 +728,8 @@ int s3d_linear_int8(const int8_t *x, const float *x_scales, const int8_t *w, con
 /*
  * Both layers of an MLP: u = fp16(GELU(x w1^T + b1)), in eight bits as s3d_quantize_rows has them, then y = u w2^T + b2, fp16
  * [M,C], with the bits of those calls one after the other.  C and hidden multiples of 16, at most 8192.  No workspace (0 bytes, null) where
- * both layers run as one kernel.
+ * both layers run as one kernel.  s3d_mlp, the layers in fp16, takes less time for the rows and widths that it is for: from 16,384 rows and 192 C
+ * on, 48 to 192 channels, up to 1024 hidden ones (149,993 rows of 160 over 640, us, 101 / 144).
  */
 size_t s3d_mlp_int8_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
 int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const float *w1_scales, const float *b1, const int8_t *w2,
@@ -786,6 +787,8 @@ int s3d_kept_linear_grad(const void *dy, const void *w_t, const void *kept, void
  * An MLP likewise: h = x w1^T + b1 (rounded to fp16), y = GELU(h) w2^T + b2, x and h kept, w1_t [C,hidden] and w2_t [hidden,C] made (each
  * unless null); dtypes HOST [4], of w1, b1, w2, b2 (that of a bias which is null is not read, but 0 or 1).  Its gradients, h' and x' what is kept:
  * dh = (dy w2) GELU'(h'), dw2 = dy^T GELU(h'), db2 = column sums of dy, dx = dh w1, dw1 = dh^T x', db1 = column sums of dh, each unless null.
+ * The operands of products are fp16 numbers: GELU(h), GELU(h') and, for dx and dw1, dh are rounded to fp16, as the layers one by one in fp16 have
+ * them.  y, dx, dw1 and dw2 are some 2.9 10^-4 of their norm off by that, a single rounding is 2.1.  db1 is the sum of dh before it is rounded.
  */
 size_t s3d_kept_mlp_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
 int s3d_kept_mlp(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, const int32_t *dtypes, void *y, void *kept_x,

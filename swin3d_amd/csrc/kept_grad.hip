@@ -10,8 +10,8 @@
 // A workgroup has 128 or 64 columns of dY by 32 B of X and a share of the rows; its eight wavefronts have 32 columns of dY each, all of X's, and
 // every second or fourth block of 32 rows.  The shares' parts are added by linear_grad.hip's second kernel: no atomics, the same bits on every call.
 //
-// Bound by memory where the widths are small (199,327 rows of 144 and 48 channels 19.9 us, 3.4 TB/s; 149,993 of 640 and 160 102 us kept, 85 in fp16, 2.1
-// and 2.8 TB/s, with dY read for every 96 of X's columns in the first), by launch and sums where rows are few (811 of 1152 and 384 12.3 us).
+// Bound by memory where the widths are small (199,327 rows of 144 and 48 channels 19.5 us, 3.5 TB/s; 149,993 of 640 and 160 96 us kept, 85 in fp16, 2.3
+// and 2.8 TB/s, with dY read for every 96 of X's columns in the first), by launch and sums where rows are few (811 of 1152 and 384 10.9 us).
 #include "attn_kernels.h"
 #include "linear.h"
 #include "rows8.h"

@@ -9,8 +9,9 @@
 // v_permlane32_swap); weights come through LDS, the next ones on their way meanwhile.  A lane has numbers 8 g + 4 half .. + 3 of 32 hidden
 // channels of its row; sixteen channels, a group of the kept form, are in a row's two lanes.
 //
-// Bound by instructions, of GELU, its derivative and the codes, and by what leaves: 149,993 rows of 160 over 640 forward 165 us (0.37 of 1.36 PFLOP/s, 1.4
-// TB/s; without codes 25 less), backward 227 (2.6 TB/s; dh's sums in fp32 are 1 to 4% of the call).
+// Bound by instructions, of GELU, its derivative and the codes, and by what leaves: 149,993 rows of 160 over 640 forward 138 us (0.45 of 1.36 PFLOP/s, 1.6
+// TB/s), backward 201 (3.0 TB/s; dh's sums in fp32 are 1 to 4% of the call), passes one after the other; the first twenty on an idle card take up to a fifth
+// longer, 165 and 227, the forward without codes 25 less, and it is there that the backward's kernel was timed without its stores (below).
 #include "attn_kernels.h"
 #include "linear.h"
 #include "rows8.h"
@@ -304,6 +305,7 @@ template <int C, Way kWay> int launch(const KeptMlp &a, hipStream_t stream)
     return S3D_OK;
 }
 
+// (a kernel a width: its sums are so many registers.  The levels' widths of Swin3D-S and -L, 64 and 128; all others take two products.)
 bool takes(int32_t C, int32_t hidden)
 {
     const bool width = C == 48 || C == 64 || C == 80 || C == 96 || C == 128 || C == 160 || C == 192;

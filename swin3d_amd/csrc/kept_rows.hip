@@ -52,7 +52,8 @@ __global__ __launch_bounds__(kThreads) void kept_values_kernel(const uint8_t *__
 }
 
 // Parameters as the products read them: fp16 copies of those in fp32, and transposed ones of weights.  Tiles of 64 x 64 that turn in LDS;
-// a bias is a matrix of one row.  One launch for all copies of a call, and bound by it (4 to 6 us for weights of up to 1152 x 384).
+// a bias is a matrix of one row.  One launch for all copies of a call (4 to 5 us for weights of up to 640 x 160, bound by it; 6 to 8, at times 12, for 1152 x 384
+// in fp32, both copies of which are 3.5 MB to read and write).
 constexpr int kSquare = 64, kMostCopies = 4;
 struct Copies {
     const void *from[kMostCopies];

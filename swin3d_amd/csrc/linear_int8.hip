@@ -6,9 +6,9 @@
 // loads, and a step of v_mfma_i32_32x32x32_i8 takes 32 of them, sixteen (a piece of 16 bytes) from each half of the lanes.  K is a
 // multiple of 16: where half a step is left, the upper lanes put in zeros.
 //
-// Short sums are bound by the rows' memory (149,993 rows, 160 to 480, 46 us, 3.7 TB/s; 199,327, 48 to 192 with GELU, 27.9, 3.1, GELU's instructions beside
-// it), long ones by LDS and the wait for a chunk (37,499, 1280 to 320, 27.3 us, 1.1 of 2.1 POP/s that a large product reaches), few rows by one tile's chunks
-// one after the other (390, 640 to 1920, 5.2 us).
+// Short sums are bound by the rows' memory (149,993 rows, 160 to 480, 42 us, 4.0 TB/s; 199,327, 48 to 192 with GELU, 26.8, 3.2, GELU's instructions beside
+// it), long ones by LDS and the wait for a chunk (37,499, 1280 to 320, 26.2 us, 1.2 of 2.1 POP/s that a large product reaches), few rows by one tile's chunks
+// one after the other (390, 640 to 1920, 5.1 us).
 #include "attn_kernels.h"
 #include "dense.h"
 #include "linear.h"

@@ -94,8 +94,10 @@ extern "C" __attribute__((visibility("default"))) int s3d_swin_blocks(
 
 // The same with the rows in front of every dense layer in eight bits: per block
 //   norm, qkv, attention (in fp16, as q, k, v are), its rows in eight bits, proj, add + norm, and the MLP
-// An MLP whose layers run as one kernel in fp16 (mlp.hip) stays that, since it writes no hidden layer: fp16 / eight bits, hidden = 4 C, 13.7 / 24.7 us
-// at 20,000 rows of 80, 50.7 / 57.3 at 37,499 of 192, 98 / 177 at 149,993 of 160, 130 / 310 at 595,677 of 80, 181 / 287 at 200,000 of 192.
+// An MLP whose layers run as one kernel in fp16 (mlp.hip) stays that: us, fp16 / eight bits (mlp_int8.hip), hidden = 4 C, 14.2 / 17.3 at 20,000 rows of 80,
+// 53.3 / 54.2 at 37,499 of 192, 101 / 144 at 149,993 of 160, 137 / 232 at 595,677 of 80, 185 / 228 at 200,000 of 192; with the norm ahead of it 19.4 / 23.3,
+// 65.6 / 69.9, 151 / 193, 234 / 334, 259 / 301.  At the line (16,384 rows or 192 C), norm and MLP: 48 channels 12.0 / 12.3, 64 14.1 / 12.9, 80 18.3 / 16.0, 96 20.3 / 22.8, 128 29.3 / 29.8, 160 38.7 / 44.3,
+// 192 64.4 / 69.7; at half of it eight bits take 0.72 to 1.05 of fp16's time, at twice 1.03 to 1.28.
 extern "C" __attribute__((visibility("default"))) size_t s3d_swin_blocks_int8_workspace_bytes(int64_t N, int32_t C, int32_t hidden)
 {
     using namespace s3d;
