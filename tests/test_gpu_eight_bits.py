@@ -434,3 +434,14 @@ def test_sum_in_place_is_a_change_that_autograd_sees(hip_lib, call):
             y.sum().backward()
     with torch.inference_mode():
         call(torch.randn(4, 48, device="cuda"), residual, norm, inplace=True)
+
+
+def test_rows_that_lack_a_part(hip_lib):
+    rows, w1, w2 = (quantize_rows(torch.randn(n, k, device="cuda")) for n, k in ((4, 48), (64, 48), (48, 64)))
+    lacking = [Int8Rows(r.codes, None) for r in (rows, w1, w2)] + [Int8Rows(None, r.scales) for r in (rows, w1, w2)]
+    for i in (0, 3):
+        for call in (lambda: lacking[i].values(), lambda: linear_int8(lacking[i], w1), lambda: linear_int8(rows, lacking[i + 1]),
+                     lambda: mlp_int8(lacking[i], w1, None, w2, None), lambda: mlp_int8(rows, lacking[i + 1], None, w2, None),
+                     lambda: mlp_int8(rows, w1, None, lacking[i + 2], None)):
+            with pytest.raises(ValueError):
+                call()
