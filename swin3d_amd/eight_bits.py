@@ -43,8 +43,9 @@ class Int8Rows(NamedTuple):
     def values(self, dtype=torch.float16):
         """[N,C] in float16 or float32: what the rows stand for.  No autograd."""
         codes, scales = self
-        if not (isinstance(codes, torch.Tensor) and codes.is_cuda and scales is not None and _ready(codes.device, codes, scales) and codes.dtype is torch.int8 and codes.dim() == 2
-                and scales.dtype is torch.float32 and scales.shape == codes.shape[:1] and codes.shape[0] <= 0x7fffffff):
+        if not (isinstance(codes, torch.Tensor) and codes.is_cuda and scales is not None and _ready(codes.device, codes, scales)
+                and codes.dtype is torch.int8 and codes.dim() == 2 and scales.dtype is torch.float32 and scales.shape == codes.shape[:1]
+                and codes.shape[0] <= 0x7fffffff):
             _check_rows("rows", self)
             codes, scales = _dense(codes), _dense(scales)
         if dtype not in _DTYPE_CODE:
@@ -213,8 +214,8 @@ def _product_operands(rows, weight, bias):
     if isinstance(rows, tuple) and isinstance(weight, tuple) and len(rows) == len(weight) == 2:
         (x, sx), (w, sw) = rows, weight
         # (the usual operands: each is looked at once)
-        if isinstance(x, torch.Tensor) and x.is_cuda and sx is not None and w is not None and sw is not None and _ready(x.device, x, sx, w, sw, bias) and x.dtype is w.dtype is torch.int8 \
-                and sx.dtype is sw.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32):
+        if isinstance(x, torch.Tensor) and x.is_cuda and sx is not None and w is not None and sw is not None \
+                and _ready(x.device, x, sx, w, sw, bias) and x.dtype is w.dtype is torch.int8 and sx.dtype is sw.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32):
             a, b = x.shape, w.shape
             if len(a) == len(b) == 2 and a[1] == b[1] and sx.shape == a[:1] and sw.shape == b[:1] and (bias is None or bias.shape == b[:1]) \
                     and a[0] <= 0x7fffffff:
