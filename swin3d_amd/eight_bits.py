@@ -78,8 +78,11 @@ def _check(name, t, dtypes, shape, device=None):
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
     sizes = t.shape
-    if not t.is_cuda or t.dtype not in dtypes or len(sizes) != len(shape) or any(s is not None and s != got for s, got in zip(shape, sizes)) \
-            or (device is not None and t.device != device):
+    fits = t.is_cuda and t.dtype in dtypes and len(sizes) == len(shape) and (device is None or t.device == device)
+    if fits:
+        for size, got in zip(shape, sizes):
+            fits = fits and (size is None or size == got)
+    if not fits:
         wanted = ",".join("any" if s is None else str(s) for s in shape)
         kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         where = "on a CUDA (HIP) device" if device is None else f"on {device}"
