@@ -728,8 +728,8 @@ int s3d_linear_int8(const int8_t *x, const float *x_scales, const int8_t *w, con
 /*
  * Both layers of an MLP: u = fp16(GELU(x w1^T + b1)), in eight bits as s3d_quantize_rows has them, then y = u w2^T + b2, fp16
  * [M,C], with the bits of those calls one after the other.  C and hidden multiples of 16, at most 8192.  No workspace (0 bytes, null) where
- * both layers run as one kernel.  s3d_mlp, the layers in fp16, takes less time for the rows and widths that it is for: from 16,384 rows and 192 C
- * on, 48 to 192 channels, up to 1024 hidden ones (149,993 rows of 160 over 640, us, 101 / 144).
+ * both layers run as one kernel.  s3d_mlp, the layers in fp16 at 48 to 192 channels over up to 1024, takes less time with many rows: from some
+ * 16,384 and 192 C on, at 64 and 80 channels from twice that (149,993 rows of 160 over 640, us, 101 / 144).
  */
 size_t s3d_mlp_int8_workspace_bytes(int64_t M, int32_t C, int32_t hidden);
 int s3d_mlp_int8(const int8_t *x, const float *x_scales, const int8_t *w1, const float *w1_scales, const float *b1, const int8_t *w2,
