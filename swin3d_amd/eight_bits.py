@@ -218,7 +218,8 @@ def _product_operands(rows, weight, bias):
         (x, sx), (w, sw) = rows, weight
         # (the usual operands: each is looked at once)
         if isinstance(x, torch.Tensor) and x.is_cuda and sx is not None and w is not None and sw is not None \
-                and _ready(x.device, x, sx, w, sw, bias) and x.dtype is w.dtype is torch.int8 and sx.dtype is sw.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32):
+                and _ready(x.device, x, sx, w, sw, bias) and x.dtype is w.dtype is torch.int8 \
+                and sx.dtype is sw.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32):
             a, b = x.shape, w.shape
             if len(a) == len(b) == 2 and a[1] == b[1] and sx.shape == a[:1] and sw.shape == b[:1] and (bias is None or bias.shape == b[:1]) \
                     and a[0] <= 0x7fffffff:
